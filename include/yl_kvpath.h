@@ -81,6 +81,8 @@ typedef enum yl_status {
 #define YL_DEVERR_POOL_EMPTY      0x1000u /* reserve: fewer free pages than the batch needs  */
 #define YL_DEVERR_POOL_OVERFLOW   0x2000u /* release: more pages than the free list holds    */
 #define YL_DEVERR_DUPLICATE_ROW   0x4000u /* reserve, release: one table row named twice     */
+#define YL_DEVERR_NONFINITE       0x8000u /* quantised store: an infinity or NaN among the new rows */
+#define YL_DEVERR_SCALE           0x20000u /* quantised pool: a scale that is not positive and finite */
 
 /*
  * Store (replaces yllang::StoreKVCache<kElementSize>,
@@ -392,6 +394,182 @@ typedef struct yl_ranges_args {
 } yl_ranges_args;
 
 YL_API int yl_make_2d_indices(const yl_ranges_args *args, cudaStream_t stream);
+
+/*
+ * 8-bit pool: K and V held as e4m3 codes with one fp32 scale for each page and
+ * KV head, value = code * scale.  Strides are free, so a page may be stored
+ * token-major or head-major; the (page, head) block that shares a scale is
+ * contiguous when slot_stride == head_dim, which is what the attention kernels
+ * read fastest.  Strides of codes are in bytes (= elements), of scales in
+ * elements; K and V share them.  No counterpart in the reference, whose pool
+ * holds 16-bit rows (src/include/kvcache/mha_kvcache.h:42-62).
+ */
+typedef struct yl_quant_pool {
+  void *k_codes;              /* e4m3 [layers, num_pages, page_size, num_heads, head_dim] */
+  void *v_codes;
+  float *k_scale;             /* [layers, num_pages, num_heads]                    */
+  float *v_scale;
+  int64_t layer_stride;       /* bytes between layers (ignored for one layer)      */
+  int64_t page_stride;        /* bytes between pages                               */
+  int64_t slot_stride;        /* bytes between the slots of a page                 */
+  int64_t head_stride;        /* bytes between the heads of a slot                 */
+  int64_t scale_layer_stride; /* elements between layers of a scale tensor         */
+  int64_t scale_page_stride;  /* elements between pages                            */
+  int64_t scale_head_stride;  /* elements between heads                            */
+  int64_t num_pages;          /* page ids are checked against it; >= 1             */
+  int32_t page_size;          /* tokens per page                                   */
+  int32_t num_heads;          /* KV heads                                          */
+  int32_t head_dim;           /* 64, 128 or 256                                    */
+  int32_t num_layers;         /* >= 1                                              */
+} yl_quant_pool;
+
+/*
+ * Quantising store: the new K/V rows of a batch, written into the 8-bit pool
+ * where the page arrays of yl_build_index put them.  Sequence i has total =
+ * (np - 1) * page_size + kv_last_page_len[i] tokens, np = kv_indptr[i + 1] -
+ * kv_indptr[i]; its last new = qo_indptr[i + 1] - qo_indptr[i] tokens are rows
+ * qo_indptr[i] .. of k and v.  For each layer, each of K and V, each page that
+ * gets new tokens and each head, with `held` the tokens that the page had:
+ *     amax  = largest finite |x| of the page's new tokens of this head
+ *     need  = 2^ceil(log2(amax / 448)), its exponent kept in [-100, 120]
+ *             (2^-100 if amax is 0)
+ *     scale = held > 0 ? max(need, scale) : need
+ *     code  = e4m3(x / scale), to nearest even, for the new tokens; an infinity
+ *             becomes +-448 and NaN e4m3's NaN, both set YL_DEVERR_NONFINITE
+ * and where the scale has grown, the held tokens take it: code = e4m3(code *
+ * old scale / scale).  Powers of two make that exact but for e4m3's subnormals,
+ * and cost no precision, since e4m3 carries an exponent of its own.  A held
+ * page whose scale is not positive and finite sets YL_DEVERR_SCALE and takes
+ * the new tokens' scale, its codes unchanged.
+ *
+ * Pages outside [0, num_pages) set YL_DEVERR_PAGE_RANGE, entries past
+ * kv_indices_capacity YL_DEVERR_INDICES_CAP, rows past num_tokens
+ * YL_DEVERR_TOKEN_COUNT, more new tokens than the sequence's pages hold
+ * YL_DEVERR_ROW_OVERFLOW; each skips those rows.  Rows behind qo_indptr[B] are
+ * not read.  A page that two sequences of one call write is outside the
+ * contract.  Row pointers and strides of k and v are multiples of 16 bytes,
+ * codes of 8.
+ */
+typedef struct yl_quant_store_args {
+  yl_quant_pool pool;
+  const void *k;              /* [layers, num_tokens, num_heads, head_dim] bf16 or fp16 */
+  const void *v;
+  const int32_t *kv_indptr;   /* [batch_size + 1]                                  */
+  const int32_t *kv_indices;  /* [kv_indices_capacity] page ids                    */
+  const int32_t *kv_last_page_len; /* [batch_size]                                 */
+  const int32_t *qo_indptr;   /* [batch_size + 1]                                  */
+  int64_t kv_indices_capacity;
+  int64_t num_tokens;         /* rows of k and v in a layer                        */
+  int64_t k_row_stride;       /* bytes between tokens                              */
+  int64_t v_row_stride;
+  int64_t k_layer_stride;     /* bytes between layers (ignored for one layer)      */
+  int64_t v_layer_stride;
+  int32_t batch_size;
+  int32_t dtype;              /* YL_DTYPE_BF16 or YL_DTYPE_F16                     */
+  uint32_t *error_word;
+} yl_quant_store_args;
+
+YL_API int yl_kv_quant_store(const yl_quant_store_args *args, cudaStream_t stream);
+
+/*
+ * Reading an 8-bit pool back: for each layer and i < num_tokens,
+ *     k_out[i, h] = T(k_code[slots[i], h] * k_scale[page of slots[i], h])
+ * and V likewise, slot = page * page_size + offset.  A value past T's range
+ * comes back as T's largest; NaN stays NaN.  Slot -1 gives a zero row, any
+ * other slot outside the pool a zero row and YL_DEVERR_SLOT_RANGE.  Output
+ * pointers and strides are multiples of 16 bytes, codes and their strides of 16.
+ */
+typedef struct yl_quant_load_args {
+  yl_quant_pool pool;
+  void *k_out;                /* [layers, num_tokens, num_heads, head_dim] bf16 or fp16 */
+  void *v_out;
+  const void *slots;          /* [num_tokens] int32 or int64                       */
+  int64_t num_tokens;
+  int64_t k_row_stride;       /* bytes between tokens of k_out                     */
+  int64_t v_row_stride;
+  int64_t k_layer_stride;     /* bytes between layers (ignored for one layer)      */
+  int64_t v_layer_stride;
+  int32_t slot_is_int64;
+  int32_t dtype;              /* YL_DTYPE_BF16 or YL_DTYPE_F16                     */
+  uint32_t *error_word;
+} yl_quant_load_args;
+
+YL_API int yl_kv_quant_load(const yl_quant_load_args *args, cudaStream_t stream);
+
+/*
+ * Paged attention of a batch's new tokens, causal from each sequence's end,
+ * over a 16-bit or an 8-bit pool, with an optional sliding window and first
+ * tokens that stay visible.  Sequence i has total and new tokens as for the
+ * quantising store; its query t (row qo_indptr[i] + t) is at position p =
+ * total - new + t and sees the key positions
+ *     j <= p  and  (window == 0  or  j > p - window  or  j < sinks).
+ * For each query head h, over KV head h / (num_q_heads / num_kv_heads):
+ *     o = sum_j softmax_j(sm_scale * q . k_j) v_j,
+ * zero where no position is seen.  Values that are not seen never reach the
+ * result, whatever they hold; pages none of whose positions a query of the
+ * sequence sees are not read, and their entries of kv_indices may hold
+ * anything (a window's pages can be given back while their entries stay).
+ * Where a query sees a V row that holds an infinity or NaN, any element of
+ * its result may be NaN.  Any number of new tokens per sequence, none
+ * included, and any page size.  Rows of o behind qo_indptr[B] stay as they were.
+ *
+ * A seen page outside [0, num_pages) sets YL_DEVERR_PAGE_RANGE and counts as
+ * not seen, entries past kv_indices_capacity YL_DEVERR_INDICES_CAP likewise;
+ * rows past num_tokens set YL_DEVERR_TOKEN_COUNT and are skipped, as are the
+ * rows of a sequence of more than max_new_len (> 0) new tokens; a sequence of
+ * 2^31 tokens or more sets YL_DEVERR_INDPTR_OVERFLOW and gives zero rows.
+ *
+ * workspace: yl_paged_attention_workspace() bytes of device memory, 16-byte
+ * aligned, whose contents need not survive or be cleared between calls; calls
+ * that may overlap on the GPU need one each.  All pointers and strides of q,
+ * o and the pool are multiples of 16 bytes.
+ */
+#define YL_KV_SAME 0  /* the pool holds `dtype` */
+#define YL_KV_E4M3 1  /* 8-bit pool with scales */
+typedef struct yl_paged_attention_args {
+  const void *q;              /* [num_tokens, num_q_heads, head_dim]               */
+  void *o;                    /* [num_tokens, num_q_heads, head_dim]               */
+  const void *k_cache;        /* one layer [num_pages, page_size, num_kv_heads, head_dim] */
+  const void *v_cache;
+  const float *k_scale;       /* [num_pages, num_kv_heads] of an 8-bit pool        */
+  const float *v_scale;
+  const int32_t *kv_indptr;   /* [batch_size + 1]                                  */
+  const int32_t *kv_indices;  /* [kv_indices_capacity]                             */
+  const int32_t *kv_last_page_len; /* [batch_size]                                 */
+  const int32_t *qo_indptr;   /* [batch_size + 1]                                  */
+  void *workspace;
+  int64_t workspace_bytes;
+  int64_t q_row_stride;       /* bytes                                             */
+  int64_t q_head_stride;
+  int64_t o_row_stride;
+  int64_t o_head_stride;
+  int64_t page_stride;        /* bytes, of both pools                              */
+  int64_t slot_stride;
+  int64_t head_stride;
+  int64_t scale_page_stride;  /* elements                                          */
+  int64_t scale_head_stride;
+  int64_t kv_indices_capacity;
+  int64_t num_pages;
+  int64_t num_tokens;         /* rows of q and o                                   */
+  int32_t batch_size;
+  int32_t num_q_heads;        /* a multiple of num_kv_heads                        */
+  int32_t num_kv_heads;
+  int32_t head_dim;           /* 64, 128 or 256                                    */
+  int32_t page_size;
+  int32_t dtype;              /* YL_DTYPE_BF16 or YL_DTYPE_F16: q and o            */
+  int32_t kv_dtype;           /* YL_KV_SAME or YL_KV_E4M3                          */
+  int32_t window;             /* 0: none                                           */
+  int32_t sinks;              /* first positions that stay visible beside a window */
+  int32_t max_new_len;        /* most new tokens of one sequence; 0: not known     */
+  float sm_scale;             /* usually 1 / sqrt(head_dim)                        */
+  uint32_t *error_word;
+} yl_paged_attention_args;
+
+YL_API int yl_paged_attention(const yl_paged_attention_args *args, cudaStream_t stream);
+
+/* Workspace bytes of a call with these sizes on the current device (the
+ * pointers of args are not looked at), or a negative yl_status. */
+YL_API int64_t yl_paged_attention_workspace(const yl_paged_attention_args *args);
 
 /* Human-readable name of a yl_status value (static storage). */
 YL_API const char *yl_status_string(int status);

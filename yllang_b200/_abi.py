@@ -35,6 +35,8 @@ DEVERR_POSITION_RANGE = 0x800
 DEVERR_POOL_EMPTY = 0x1000
 DEVERR_POOL_OVERFLOW = 0x2000
 DEVERR_DUPLICATE_ROW = 0x4000
+DEVERR_NONFINITE = 0x8000
+DEVERR_SCALE = 0x20000
 
 ABI_VERSION = 1
 
@@ -221,9 +223,121 @@ class RangesArgs(ctypes.Structure):
     ]
 
 
+class QuantPool(ctypes.Structure):
+    """struct yl_quant_pool."""
+
+    _fields_ = [
+        ("k_codes", _vp),
+        ("v_codes", _vp),
+        ("k_scale", _vp),
+        ("v_scale", _vp),
+        ("layer_stride", _i64),
+        ("page_stride", _i64),
+        ("slot_stride", _i64),
+        ("head_stride", _i64),
+        ("scale_layer_stride", _i64),
+        ("scale_page_stride", _i64),
+        ("scale_head_stride", _i64),
+        ("num_pages", _i64),
+        ("page_size", _i32),
+        ("num_heads", _i32),
+        ("head_dim", _i32),
+        ("num_layers", _i32),
+    ]
+
+
+class QuantStoreArgs(ctypes.Structure):
+    """struct yl_quant_store_args."""
+
+    _fields_ = [
+        ("pool", QuantPool),
+        ("k", _vp),
+        ("v", _vp),
+        ("kv_indptr", _vp),
+        ("kv_indices", _vp),
+        ("kv_last_page_len", _vp),
+        ("qo_indptr", _vp),
+        ("kv_indices_capacity", _i64),
+        ("num_tokens", _i64),
+        ("k_row_stride", _i64),
+        ("v_row_stride", _i64),
+        ("k_layer_stride", _i64),
+        ("v_layer_stride", _i64),
+        ("batch_size", _i32),
+        ("dtype", _i32),
+        ("error_word", _vp),
+    ]
+
+
+class QuantLoadArgs(ctypes.Structure):
+    """struct yl_quant_load_args."""
+
+    _fields_ = [
+        ("pool", QuantPool),
+        ("k_out", _vp),
+        ("v_out", _vp),
+        ("slots", _vp),
+        ("num_tokens", _i64),
+        ("k_row_stride", _i64),
+        ("v_row_stride", _i64),
+        ("k_layer_stride", _i64),
+        ("v_layer_stride", _i64),
+        ("slot_is_int64", _i32),
+        ("dtype", _i32),
+        ("error_word", _vp),
+    ]
+
+
+YL_KV_SAME, YL_KV_E4M3 = 0, 1
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """struct yl_paged_attention_args."""
+
+    _fields_ = [
+        ("q", _vp),
+        ("o", _vp),
+        ("k_cache", _vp),
+        ("v_cache", _vp),
+        ("k_scale", _vp),
+        ("v_scale", _vp),
+        ("kv_indptr", _vp),
+        ("kv_indices", _vp),
+        ("kv_last_page_len", _vp),
+        ("qo_indptr", _vp),
+        ("workspace", _vp),
+        ("workspace_bytes", _i64),
+        ("q_row_stride", _i64),
+        ("q_head_stride", _i64),
+        ("o_row_stride", _i64),
+        ("o_head_stride", _i64),
+        ("page_stride", _i64),
+        ("slot_stride", _i64),
+        ("head_stride", _i64),
+        ("scale_page_stride", _i64),
+        ("scale_head_stride", _i64),
+        ("kv_indices_capacity", _i64),
+        ("num_pages", _i64),
+        ("num_tokens", _i64),
+        ("batch_size", _i32),
+        ("num_q_heads", _i32),
+        ("num_kv_heads", _i32),
+        ("head_dim", _i32),
+        ("page_size", _i32),
+        ("dtype", _i32),
+        ("kv_dtype", _i32),
+        ("window", _i32),
+        ("sinks", _i32),
+        ("max_new_len", _i32),
+        ("sm_scale", ctypes.c_float),
+        ("error_word", _vp),
+    ]
+
+
 # Every symbol include/yl_kvpath.h declares.
 EXPORTED_SYMBOLS = ("yl_kv_store", "yl_build_index", "yl_kv_step", "yl_gather_rows", "yl_qkv_norm_rope_store",
-                    "yl_reserve_pages", "yl_release_pages", "yl_make_2d_indices", "yl_status_string", "yl_last_error",
+                    "yl_reserve_pages", "yl_release_pages", "yl_make_2d_indices", "yl_kv_quant_store", "yl_kv_quant_load",
+                    "yl_paged_attention", "yl_paged_attention_workspace", "yl_status_string", "yl_last_error",
                     "yl_abi_version")
 
 _lib: ctypes.CDLL | None = None
@@ -262,6 +376,14 @@ def lib() -> ctypes.CDLL:
         L.yl_release_pages.argtypes = [ctypes.POINTER(ReleaseArgs), _vp]
         L.yl_make_2d_indices.restype = ctypes.c_int
         L.yl_make_2d_indices.argtypes = [ctypes.POINTER(RangesArgs), _vp]
+        L.yl_kv_quant_store.restype = ctypes.c_int
+        L.yl_kv_quant_store.argtypes = [ctypes.POINTER(QuantStoreArgs), _vp]
+        L.yl_kv_quant_load.restype = ctypes.c_int
+        L.yl_kv_quant_load.argtypes = [ctypes.POINTER(QuantLoadArgs), _vp]
+        L.yl_paged_attention.restype = ctypes.c_int
+        L.yl_paged_attention.argtypes = [ctypes.POINTER(PagedAttentionArgs), _vp]
+        L.yl_paged_attention_workspace.restype = _i64
+        L.yl_paged_attention_workspace.argtypes = [ctypes.POINTER(PagedAttentionArgs)]
         L.yl_status_string.restype = ctypes.c_char_p
         L.yl_status_string.argtypes = [ctypes.c_int]
         L.yl_last_error.restype = ctypes.c_char_p
@@ -317,3 +439,19 @@ def release_pages_raw(args: ReleaseArgs, stream: int | None) -> int:
 
 def make_2d_indices_raw(args: RangesArgs, stream: int | None) -> int:
     return lib().yl_make_2d_indices(ctypes.byref(args), stream)
+
+
+def kv_quant_store_raw(args: QuantStoreArgs, stream: int | None) -> int:
+    return lib().yl_kv_quant_store(ctypes.byref(args), stream)
+
+
+def kv_quant_load_raw(args: QuantLoadArgs, stream: int | None) -> int:
+    return lib().yl_kv_quant_load(ctypes.byref(args), stream)
+
+
+def paged_attention_raw(args: PagedAttentionArgs, stream: int | None) -> int:
+    return lib().yl_paged_attention(ctypes.byref(args), stream)
+
+
+def paged_attention_workspace_raw(args: PagedAttentionArgs) -> int:
+    return lib().yl_paged_attention_workspace(ctypes.byref(args))

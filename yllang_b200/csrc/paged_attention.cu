@@ -1,0 +1,234 @@
+// Paged attention over a 16-bit or an 8-bit pool, causal from each sequence's
+// end, with an optional sliding window and first tokens that stay visible.
+//
+// One warp per (new token, query head): the lanes split the head dimension and
+// the warp walks the visible positions with a running maximum and sum.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "common.cuh"
+#include "quant_device.cuh"
+
+namespace ylk {
+namespace {
+
+struct AttnParams {
+  const char *q;
+  char *o;
+  const char *kv[2];
+  const float *scale[2];
+  const int32_t *kv_indptr, *kv_indices, *last_len, *qo_indptr;
+  int64_t q_row_stride, q_head_stride, o_row_stride, o_head_stride;
+  int64_t page_stride, slot_stride, head_stride;
+  int64_t scale_page_stride, scale_head_stride;
+  int64_t indices_cap;
+  int64_t num_tokens;
+  uint32_t *error_word;
+  int32_t num_pages, batch, heads, group, page_size, window, sinks, max_new;
+  float scale_log2;
+};
+
+constexpr int kSimpleWarps = 4;
+
+template <typename T, bool Q8, int N>
+__device__ __forceinline__ void load_row(const char *at, float scale, float (&x)[N]) {
+  if (Q8) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint16_t c = *reinterpret_cast<const uint16_t *>(at + i);
+      const float2 f = half2_bits_to_float2(e4m3x2_to_half2(c));
+      x[i] = f.x * scale;
+      x[i + 1] = f.y * scale;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 f = T::unpack(*reinterpret_cast<const uint32_t *>(at + 2 * i));
+      x[i] = f.x;
+      x[i + 1] = f.y;
+    }
+  }
+}
+
+template <typename T, int D, bool Q8>
+__global__ void __launch_bounds__(kSimpleWarps * 32) attend_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int N = D / 32;
+  constexpr int kItem = Q8 ? 1 : 2;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.x;
+  const int kvh = blockIdx.y;
+  pdl_wait();
+  const int i = warp_find(p.batch, row, lane, [&](int s) -> int64_t { return __ldg(p.qo_indptr + s); });
+  const int64_t q0 = __ldg(p.qo_indptr + i), q1 = __ldg(p.qo_indptr + i + 1);
+  const int64_t e0 = __ldg(p.kv_indptr + i), pages = static_cast<int64_t>(__ldg(p.kv_indptr + i + 1)) - e0;
+  if (row < q0 || row >= q1) return;  // behind the last sequence
+  const int64_t fresh = q1 - q0;
+  const bool report = threadIdx.x == 0 && kvh == 0;
+  if (p.max_new > 0 && fresh > p.max_new) {
+    if (report) raise_deverr(p.error_word, YL_DEVERR_TOKEN_COUNT);
+    return;
+  }
+  if (report && q1 > p.num_tokens) raise_deverr(p.error_word, YL_DEVERR_TOKEN_COUNT);
+  const int last = min(max(__ldg(p.last_len + i), 0), p.page_size);
+  int64_t total = pages > 0 ? (pages - 1) * p.page_size + last : 0;
+  if (total >= (1ll << 31)) {
+    if (report) raise_deverr(p.error_word, YL_DEVERR_INDPTR_OVERFLOW);
+    total = 0;
+  }
+  const int pos = static_cast<int>(max(total - fresh + (row - q0), int64_t(-1)));
+  const int low = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+  const int head = min(p.window > 0 ? p.sinks : 0, low);
+  for (int g = threadIdx.x >> 5; g < p.group; g += kSimpleWarps) {
+    const int h = kvh * p.group + g;
+    float q[N], acc[N], m = -INFINITY, l = 0.f;
+    load_row<T, false>(p.q + row * p.q_row_stride + h * p.q_head_stride + lane * N * 2, 1.f, q);
+#pragma unroll
+    for (int d = 0; d < N; ++d) acc[d] = 0.f;
+    for (int s = 0; s < head + (pos + 1 - low); ++s) {
+      const int j = s < head ? s : low + s - head;
+      const int64_t e = e0 + j / p.page_size;
+      if (e < 0 || e >= p.indices_cap) {
+        if (report) raise_deverr(p.error_word, YL_DEVERR_INDICES_CAP);
+        continue;
+      }
+      const int64_t page = __ldg(p.kv_indices + e);
+      if (page < 0 || page >= p.num_pages) {
+        if (report) raise_deverr(p.error_word, YL_DEVERR_PAGE_RANGE);
+        continue;
+      }
+      const int64_t at = page * p.page_stride + (j % p.page_size) * p.slot_stride + kvh * p.head_stride + lane * N * kItem;
+      const int64_t sc = page * p.scale_page_stride + kvh * p.scale_head_stride;
+      float k[N], v[N], dot = 0.f;
+      load_row<T, Q8>(p.kv[0] + at, Q8 ? __ldg(p.scale[0] + sc) : 1.f, k);
+      load_row<T, Q8>(p.kv[1] + at, Q8 ? __ldg(p.scale[1] + sc) : 1.f, v);
+#pragma unroll
+      for (int d = 0; d < N; ++d) dot += q[d] * k[d];
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+      dot *= p.scale_log2;
+      const float m2 = fmaxf(m, dot);
+      const float keep = m2 == -INFINITY ? 1.f : exp2f(m - m2), w = m2 == -INFINITY ? 0.f : exp2f(dot - m2);
+      m = m2;
+      l = l * keep + w;
+#pragma unroll
+      for (int d = 0; d < N; ++d) acc[d] = acc[d] * keep + w * v[d];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    char *out = p.o + row * p.o_row_stride + h * p.o_head_stride + lane * N * 2;
+#pragma unroll
+    for (int d = 0; d < N; d += 2) *reinterpret_cast<uint32_t *>(out + 2 * d) = T::pack(acc[d] * inv, acc[d + 1] * inv);
+  }
+}
+
+int check_attention(const yl_paged_attention_args *a, bool pointers) {
+  if (a == nullptr) return fail(YL_ERR_NULL_ARG, "yl_paged_attention: args is NULL");
+  if (a->batch_size < 0) return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: batch_size=%lld < 0", a->batch_size);
+  if (a->num_tokens < 0) return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: num_tokens=%lld < 0", a->num_tokens);
+  if (a->num_tokens >= (1ll << 31))
+    return fail(YL_ERR_UNSUPPORTED, "yl_paged_attention: num_tokens=%lld must be below 2^31", a->num_tokens);
+  if (a->dtype != YL_DTYPE_BF16 && a->dtype != YL_DTYPE_F16)
+    return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: dtype=%lld unknown", a->dtype);
+  if (a->kv_dtype != YL_KV_SAME && a->kv_dtype != YL_KV_E4M3)
+    return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: kv_dtype=%lld unknown", a->kv_dtype);
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)
+    return fail(YL_ERR_UNSUPPORTED, "yl_paged_attention: head_dim=%lld must be 64, 128 or 256", a->head_dim);
+  if (a->num_kv_heads < 1 || a->num_q_heads < 1 || a->num_q_heads % a->num_kv_heads != 0)
+    return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: num_q_heads=%lld must be a multiple of num_kv_heads=%lld",
+                a->num_q_heads, a->num_kv_heads);
+  if (a->num_kv_heads > 65535)
+    return fail(YL_ERR_UNSUPPORTED, "yl_paged_attention: num_kv_heads=%lld exceeds 65535", a->num_kv_heads);
+  if (a->page_size < 1) return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: page_size=%lld < 1", a->page_size);
+  if (a->window < 0 || a->sinks < 0 || a->max_new_len < 0)
+    return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: window, sinks and max_new_len must not be negative");
+  if (!(a->sm_scale > 0.f) || !(a->sm_scale <= 3.0e38f))
+    return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: sm_scale must be positive and finite");
+  if (a->kv_indices_capacity < 0)
+    return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: kv_indices_capacity=%lld < 0", a->kv_indices_capacity);
+  if (a->num_pages < 1 || a->num_pages >= (1ll << 31))
+    return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: num_pages=%lld must be in [1, 2^31)", a->num_pages);
+  if (!pointers || a->batch_size == 0 || a->num_tokens == 0) return YL_OK;
+  const int64_t item = a->kv_dtype == YL_KV_E4M3 ? 1 : 2;
+  if (!a->q || !a->o || !a->k_cache || !a->v_cache || !a->kv_indptr || !a->kv_last_page_len || !a->qo_indptr ||
+      (!a->kv_indices && a->kv_indices_capacity > 0))
+    return fail(YL_ERR_NULL_ARG, "yl_paged_attention: q, o, the pool and the page arrays must be non-NULL");
+  if (a->kv_dtype == YL_KV_E4M3 && (!a->k_scale || !a->v_scale))
+    return fail(YL_ERR_NULL_ARG, "yl_paged_attention: an 8-bit pool needs k_scale and v_scale");
+  if (a->q_head_stride < a->head_dim * 2 || a->o_head_stride < a->head_dim * 2 || a->q_row_stride < a->head_dim * 2 ||
+      a->o_row_stride < a->head_dim * 2 || a->slot_stride < a->head_dim * item ||
+      a->head_stride < a->head_dim * item || a->page_stride < a->head_dim * item)
+    return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: strides must be at least one head row of %lld elements",
+                a->head_dim);
+  if (a->kv_dtype == YL_KV_E4M3 && (a->scale_page_stride < 1 || a->scale_head_stride < 1))
+    return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: scale strides must be positive");
+  const uintptr_t bits =
+      reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->o) | reinterpret_cast<uintptr_t>(a->k_cache) |
+      reinterpret_cast<uintptr_t>(a->v_cache) |
+      static_cast<uintptr_t>(a->q_row_stride | a->q_head_stride | a->o_row_stride | a->o_head_stride |
+                             a->page_stride | a->slot_stride | a->head_stride);
+  if (bits & 15u)
+    return fail(YL_ERR_ALIGNMENT, "yl_paged_attention: pointers and strides of q, o and the pool must be multiples of "
+                                  "16 bytes");
+  return YL_OK;
+}
+
+}  // namespace
+}  // namespace ylk
+
+extern "C" int64_t yl_paged_attention_workspace(const yl_paged_attention_args *a) {
+  using namespace ylk;
+  clear_last_error();
+  const int rc = check_attention(a, false);
+  return rc != YL_OK ? rc : 0;
+}
+
+extern "C" int yl_paged_attention(const yl_paged_attention_args *a, cudaStream_t stream) {
+  using namespace ylk;
+  clear_last_error();
+  const int rc = check_attention(a, true);
+  if (rc != YL_OK) return rc;
+  if (a->batch_size == 0 || a->num_tokens == 0) return YL_OK;
+  AttnParams p;
+  p.q = static_cast<const char *>(a->q);
+  p.o = static_cast<char *>(a->o);
+  p.kv[0] = static_cast<const char *>(a->k_cache);
+  p.kv[1] = static_cast<const char *>(a->v_cache);
+  p.scale[0] = a->k_scale;
+  p.scale[1] = a->v_scale;
+  p.kv_indptr = a->kv_indptr;
+  p.kv_indices = a->kv_indices;
+  p.last_len = a->kv_last_page_len;
+  p.qo_indptr = a->qo_indptr;
+  p.q_row_stride = a->q_row_stride;
+  p.q_head_stride = a->q_head_stride;
+  p.o_row_stride = a->o_row_stride;
+  p.o_head_stride = a->o_head_stride;
+  p.page_stride = a->page_stride;
+  p.slot_stride = a->slot_stride;
+  p.head_stride = a->head_stride;
+  p.scale_page_stride = a->scale_page_stride;
+  p.scale_head_stride = a->scale_head_stride;
+  p.indices_cap = a->kv_indices_capacity;
+  p.num_tokens = a->num_tokens;
+  p.error_word = a->error_word;
+  p.num_pages = static_cast<int32_t>(a->num_pages);
+  p.batch = a->batch_size;
+  p.heads = a->num_kv_heads;
+  p.group = a->num_q_heads / a->num_kv_heads;
+  p.page_size = a->page_size;
+  p.window = a->window;
+  p.sinks = a->sinks;
+  p.max_new = a->max_new_len;
+  p.scale_log2 = a->sm_scale * 1.44269504088896f;
+  const dim3 grid(static_cast<unsigned>(a->num_tokens), static_cast<unsigned>(a->num_kv_heads));
+  auto go = [&](auto t, auto q8) {
+    using T = decltype(t);
+    constexpr bool Q8 = decltype(q8)::value;
+    auto fn = a->head_dim == 64 ? attend_kernel<T, 64, Q8> : a->head_dim == 128 ? attend_kernel<T, 128, Q8>
+                                                                               : attend_kernel<T, 256, Q8>;
+    return launch_dependent(fn, grid, dim3(kSimpleWarps * 32), 0, stream, "yl_paged_attention launch", p);
+  };
+  const bool q8 = a->kv_dtype == YL_KV_E4M3;
+  if (a->dtype == YL_DTYPE_BF16) return q8 ? go(Bf16{}, std::true_type{}) : go(Bf16{}, std::false_type{});
+  return q8 ? go(Fp16{}, std::true_type{}) : go(Fp16{}, std::false_type{});
+}

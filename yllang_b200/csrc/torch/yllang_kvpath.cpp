@@ -39,7 +39,9 @@ std::string DeviceErrorNames(uint32_t bits) {
       {YL_DEVERR_TOKEN_COUNT, "TOKEN_COUNT"},         {YL_DEVERR_TIMEOUT, "TIMEOUT"},
       {YL_DEVERR_INDEX_RANGE, "INDEX_RANGE"},         {YL_DEVERR_POSITION_RANGE, "POSITION_RANGE"},
       {YL_DEVERR_POOL_EMPTY, "POOL_EMPTY"},           {YL_DEVERR_POOL_OVERFLOW, "POOL_OVERFLOW"},
-      {YL_DEVERR_DUPLICATE_ROW, "DUPLICATE_ROW"}};
+      {YL_DEVERR_DUPLICATE_ROW, "DUPLICATE_ROW"},
+      {YL_DEVERR_NONFINITE, "NONFINITE"},
+      {YL_DEVERR_SCALE, "SCALE"}};
   std::string out;
   for (const auto &[bit, name] : kNames) {
     if ((bits & bit) == 0) continue;
