@@ -517,7 +517,7 @@ YL_API int yl_kv_quant_load(const yl_quant_load_args *args, cudaStream_t stream)
  * not seen, entries past kv_indices_capacity YL_DEVERR_INDICES_CAP likewise;
  * rows past num_tokens set YL_DEVERR_TOKEN_COUNT and are skipped, as are the
  * rows of a sequence of more than max_new_len (> 0) new tokens; a sequence of
- * 2^31 tokens or more sets YL_DEVERR_INDPTR_OVERFLOW and gives zero rows.
+ * 2^30 tokens or more sets YL_DEVERR_INDPTR_OVERFLOW and gives zero rows.
  *
  * workspace: yl_paged_attention_workspace() bytes of device memory, 16-byte
  * aligned, whose contents need not survive or be cleared between calls; calls

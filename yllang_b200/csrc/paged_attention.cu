@@ -5,31 +5,16 @@
 // the warp walks the visible positions with a running maximum and sum.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
-#include "common.cuh"
-#include "quant_device.cuh"
+#include "attend_device.cuh"
 
 namespace ylk {
 namespace {
 
-struct AttnParams {
-  const char *q;
-  char *o;
-  const char *kv[2];
-  const float *scale[2];
-  const int32_t *kv_indptr, *kv_indices, *last_len, *qo_indptr;
-  int64_t q_row_stride, q_head_stride, o_row_stride, o_head_stride;
-  int64_t page_stride, slot_stride, head_stride;
-  int64_t scale_page_stride, scale_head_stride;
-  int64_t indices_cap;
-  int64_t num_tokens;
-  uint32_t *error_word;
-  int32_t num_pages, batch, heads, group, page_size, window, sinks, max_new;
-  float scale_log2;
-};
-
 constexpr int kSimpleWarps = 4;
+constexpr int kDecodeRows = 64;  // query rows per KV head up to which a sequence is the decode kernel's
 
 template <typename T, bool Q8, int N>
 __device__ __forceinline__ void load_row(const char *at, float scale, float (&x)[N]) {
@@ -60,23 +45,12 @@ __global__ void __launch_bounds__(kSimpleWarps * 32) attend_kernel(const __grid_
   const int kvh = blockIdx.y;
   pdl_wait();
   const int i = warp_find(p.batch, row, lane, [&](int s) -> int64_t { return __ldg(p.qo_indptr + s); });
-  const int64_t q0 = __ldg(p.qo_indptr + i), q1 = __ldg(p.qo_indptr + i + 1);
-  const int64_t e0 = __ldg(p.kv_indptr + i), pages = static_cast<int64_t>(__ldg(p.kv_indptr + i + 1)) - e0;
-  if (row < q0 || row >= q1) return;  // behind the last sequence
-  const int64_t fresh = q1 - q0;
   const bool report = threadIdx.x == 0 && kvh == 0;
-  if (p.max_new > 0 && fresh > p.max_new) {
-    if (report) raise_deverr(p.error_word, YL_DEVERR_TOKEN_COUNT);
-    return;
-  }
-  if (report && q1 > p.num_tokens) raise_deverr(p.error_word, YL_DEVERR_TOKEN_COUNT);
-  const int last = min(max(__ldg(p.last_len + i), 0), p.page_size);
-  int64_t total = pages > 0 ? (pages - 1) * p.page_size + last : 0;
-  if (total >= (1ll << 31)) {
-    if (report) raise_deverr(p.error_word, YL_DEVERR_INDPTR_OVERFLOW);
-    total = 0;
-  }
-  const int pos = static_cast<int>(max(total - fresh + (row - q0), int64_t(-1)));
+  const Seq sq = load_seq(p, i, report);
+  if (row < sq.q0 || row >= static_cast<int64_t>(sq.q0) + sq.fresh) return;  // behind the last sequence
+  if (static_cast<int64_t>(sq.fresh) * p.group <= p.max_rows) return;        // the decode kernel's
+  const int64_t e0 = sq.e0;
+  const int pos = max(sq.total - sq.fresh + static_cast<int>(row - sq.q0), -1);
   const int low = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
   const int head = min(p.window > 0 ? p.sinks : 0, low);
   for (int g = threadIdx.x >> 5; g < p.group; g += kSimpleWarps) {
@@ -136,8 +110,8 @@ int check_attention(const yl_paged_attention_args *a, bool pointers) {
   if (a->num_kv_heads < 1 || a->num_q_heads < 1 || a->num_q_heads % a->num_kv_heads != 0)
     return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: num_q_heads=%lld must be a multiple of num_kv_heads=%lld",
                 a->num_q_heads, a->num_kv_heads);
-  if (a->num_kv_heads > 65535)
-    return fail(YL_ERR_UNSUPPORTED, "yl_paged_attention: num_kv_heads=%lld exceeds 65535", a->num_kv_heads);
+  if (a->num_kv_heads > 32767)
+    return fail(YL_ERR_UNSUPPORTED, "yl_paged_attention: num_kv_heads=%lld exceeds 32767", a->num_kv_heads);
   if (a->page_size < 1) return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: page_size=%lld < 1", a->page_size);
   if (a->window < 0 || a->sinks < 0 || a->max_new_len < 0)
     return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: window, sinks and max_new_len must not be negative");
@@ -179,15 +153,20 @@ extern "C" int64_t yl_paged_attention_workspace(const yl_paged_attention_args *a
   using namespace ylk;
   clear_last_error();
   const int rc = check_attention(a, false);
-  return rc != YL_OK ? rc : 0;
+  return rc != YL_OK ? rc : decode_workspace(a);
 }
 
 extern "C" int yl_paged_attention(const yl_paged_attention_args *a, cudaStream_t stream) {
   using namespace ylk;
   clear_last_error();
-  const int rc = check_attention(a, true);
+  int rc = check_attention(a, true);
   if (rc != YL_OK) return rc;
   if (a->batch_size == 0 || a->num_tokens == 0) return YL_OK;
+  if (a->workspace == nullptr || a->workspace_bytes < decode_workspace(a))
+    return fail(a->workspace ? YL_ERR_BAD_SIZE : YL_ERR_NULL_ARG,
+                "yl_paged_attention: workspace must hold %lld bytes", decode_workspace(a));
+  if (reinterpret_cast<uintptr_t>(a->workspace) & 15u)
+    return fail(YL_ERR_ALIGNMENT, "yl_paged_attention: workspace must be 16-byte aligned");
   AttnParams p;
   p.q = static_cast<const char *>(a->q);
   p.o = static_cast<char *>(a->o);
@@ -219,7 +198,14 @@ extern "C" int yl_paged_attention(const yl_paged_attention_args *a, cudaStream_t
   p.window = a->window;
   p.sinks = a->sinks;
   p.max_new = a->max_new_len;
+  p.by_page = FastDiv(static_cast<uint32_t>(a->page_size));
+  p.by_group = FastDiv(static_cast<uint32_t>(p.group));
   p.scale_log2 = a->sm_scale * 1.44269504088896f;
+  p.max_rows = kDecodeRows;
+  // most query rows per KV head that a sequence can have
+  const int64_t most = (a->max_new_len > 0 ? std::min<int64_t>(a->max_new_len, a->num_tokens) : a->num_tokens) * p.group;
+  rc = launch_decode(p, a, most, stream);
+  if (rc != YL_OK || most <= kDecodeRows) return rc;
   const dim3 grid(static_cast<unsigned>(a->num_tokens), static_cast<unsigned>(a->num_kv_heads));
   auto go = [&](auto t, auto q8) {
     using T = decltype(t);
