@@ -15,15 +15,17 @@
 //   unit ahead, and fills a ring of stages with 16-byte asynchronous copies,
 //   across the ends of sequences.  Tokens that no query sees are zero-filled,
 //   not read.
-// * Four warps compute, 16 tokens of a stage each, with their own running
+// * Four warps compute, each on its own quarter of the tile with its own running
 //   maximum, sum and accumulator (online softmax); the four are joined when a
-//   (sequence, head) ends.  Products are m16n8k16 matrix instructions on 16
-//   query rows: at 4 to 16 rows these tiles cost less issue than the loads cost
-//   bandwidth, which a 128-row tensor tile would waste on padding.
+//   (sequence, head) ends.  Products are m16n8k16 matrix instructions with the
+//   16 rows along the tokens (k.q) or the head dimension (v.p) and 8 columns of
+//   query rows: at 1 to 16 query rows this wastes least, where a 128-row tensor
+//   tile would be padding.  The weights turn from the first product's result to
+//   the second's operand by a transposing register move.
 // * An 8-bit pool is multiplied in fp16: every e4m3 value is exact there.  bf16
 //   queries are first brought into fp16's range by a power of two per row,
 //   exact for all elements within 2^-24 of the row's largest.  The contraction
-//   order of q.k is free, so a lane takes 4 neighbouring codes as its part of a
+//   order of k.q is free, so a lane takes 4 neighbouring codes as its part of a
 //   k-step and K needs no transposition; the codes of two tokens of V are
 //   interleaved by byte permutes before conversion.  K's scale multiplies the
 //   scores; V's scale, relative to the largest seen so far, multiplies the
@@ -46,17 +48,15 @@
 namespace ylk {
 namespace {
 
-constexpr int kTile = 64;     // tokens of a unit
-constexpr int kConsumers = 4; // warps that compute, kTile / 4 tokens each
+constexpr int kConsumers = 4;  // warps that compute, a quarter of a unit's tokens each
 constexpr int kThreads = (kConsumers + 1) * 32;
-constexpr int kRows = 16;     // query rows of a unit
 // A CTA's run is at least this many units, so that a short sequence is not cut
 // into parts whose joining costs more than they save.
 constexpr int kMinRun = 2;
 
 // Unit descriptor in a stage, written by the loading warp.
 struct UnitInfo {
-  uint32_t valid[2];  // tokens of the tile that some query sees, with a good page
+  uint32_t valid[4];  // tokens of the tile that some query sees, with a good page
   int base;           // position of the tile's first token
   int flags;          // kFirst | kLast | kWhole | kRagged
   int pos0;           // position of the sequence's first query
@@ -71,21 +71,27 @@ constexpr int kLast = 2;    // last one
 constexpr int kWhole = 4;   // with kLast: this CTA has all of its units
 constexpr int kRagged = 8;  // some query does not see some valid token
 
-template <int D, bool Q8>
+// NB: blocks of 8 query rows of a unit.
+template <int D, bool Q8, int NB>
 struct Layout {
   static constexpr int kItem = Q8 ? 1 : 2;
   static constexpr int kRow = D * kItem;            // bytes of a token's head row
   static constexpr int kChunks = kRow / 16;         // 16-byte chunks of it
+  static constexpr int kTokens = kRow <= 128 ? 32 : 16;  // of a computing warp: 8 KB of K and V or less, but for kRow 512
+  static constexpr int kTile = kConsumers * kTokens;
+  static constexpr int kRows = 8 * NB;              // query rows of a unit
   static constexpr int kKV = kTile * kRow;          // bytes of K (or V) in a stage
   static constexpr int kQ = kRows * D * 2;
   static constexpr int kScales = Q8 ? 2 * kTile * 4 : 0;
-  static constexpr int kStage = 2 * kKV + kQ + kScales + 64;
-  static constexpr int kMerge = 2 * kRows * D * 4;  // two warps' accumulators
-  // two CTAs per SM where a stage is small enough for three of them each
-  static constexpr int kCtas = kStage * 3 + kMerge + 1024 <= 113 * 1024 ? 2 : 1;
-  static constexpr int kBudget = (kCtas == 2 ? 113 : 226) * 1024 - kMerge - 1024;
+  static constexpr int kInfo = 2 * kKV + kQ + kScales;
+  static constexpr int kStage = kInfo + 128;
+  static constexpr int kMerge = 2 * (kRows * D + 2 * kRows) * 4;  // two warps' accumulators, maxima and sums
+  static constexpr int kRest = 128 + 256;           // alignment of the stages, barriers
+  // two CTAs per SM where two stages and more fit each
+  static constexpr int kCtas = kStage * 2 + kMerge + kRest <= 113 * 1024 ? 2 : 1;
+  static constexpr int kBudget = (kCtas == 2 ? 113 : 226) * 1024 - kMerge - kRest;
   static constexpr int kStages = kBudget / kStage > 8 ? 8 : kBudget / kStage;
-  static constexpr int kSmem = kStages * kStage + kMerge + 1024;
+  static constexpr int kSmem = kStages * kStage + kMerge + kRest;
   static_assert(kStages >= 2, "a ring needs two stages");
 };
 
@@ -99,7 +105,7 @@ __device__ __forceinline__ int chunk_at(int r, int c) {
     return line * 128 + ((((r & 1) * 4 + c) ^ f) << 4);
   }
   const int f = Q8 ? ((((r & 1) ^ ((r >> 2) & 1)) << 2) | (r & 2)) : (r & 7);
-  return r * Layout<D, Q8>::kRow + (((c & ~7) | ((c ^ f) & 7)) << 4);
+  return r * (D * (Q8 ? 1 : 2)) + (((c & ~7) | ((c ^ f) & 7)) << 4);
 }
 
 template <bool BF>
@@ -144,20 +150,45 @@ __device__ __forceinline__ uint32_t lds32(uint32_t at) {
 __device__ __forceinline__ uint32_t e4m3_lo(uint32_t w) { return e4m3x2_to_half2(static_cast<uint16_t>(w)); }
 __device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) { return e4m3x2_to_half2(static_cast<uint16_t>(w >> 16)); }
 
-// Zero the 16-bit halves of w that hold an infinity or NaN; bit 0 / 1 of the
-// result says which did.
-template <bool BF>
-__device__ __forceinline__ uint32_t drop_nonfinite(uint32_t &w) {
-  constexpr uint32_t inf = BF ? 0x7f80u : 0x7c00u;
+// An 8 x 8 matrix of 16-bit values turned over, in the layout of a fragment.
+__device__ __forceinline__ uint32_t turn(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Zero what is no finite number in the V rows [t0, t0 + TOKENS) of a tile, so
+// that weight 0 times it is 0; returns which of the tokens had any.  Only for
+// tiles of which some query does not see all: elsewhere it belongs in the
+// result.
+template <int D, bool Q8, bool BF, int TOKENS>
+__device__ __noinline__ uint32_t clean_values(uint32_t sv, int t0) {
+  constexpr uint32_t inf = BF ? 0x7f807f80u : 0x7c007c00u;
+  constexpr int kChunks = D * (Q8 ? 1 : 2) / 16;
+  const int lane = threadIdx.x & 31;
   uint32_t bad = 0;
-  if ((w & inf) == inf) {
-    bad |= 1;
-    w &= 0xffff0000u;
+#pragma unroll 1
+  for (int n = lane; n < TOKENS * kChunks; n += 32) {
+    const int t = n % TOKENS;
+    const uint32_t at = sv + chunk_at<D, Q8>(t0 + t, n / TOKENS);
+    uint4 w = lds128(at);
+    uint32_t any = 0;
+    auto clean = [&](uint32_t &x) {
+      const uint32_t mask = Q8 ? __vcmpeq4(x & 0x7f7f7f7fu, 0x7f7f7f7fu) : __vcmpgeu2(x & 0x7fff7fffu, inf);
+      any |= mask;
+      x &= ~mask;
+    };
+    clean(w.x);
+    clean(w.y);
+    clean(w.z);
+    clean(w.w);
+    if (any) {
+      bad |= 1u << t;
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+    }
   }
-  if (((w >> 16) & inf) == inf) {
-    bad |= 2;
-    w &= 0x0000ffffu;
-  }
+  bad = __reduce_or_sync(0xffffffffu, bad);
+  __syncwarp();
   return bad;
 }
 
@@ -171,7 +202,9 @@ struct SeqWork {
   int64_t units;
 };
 
+template <class L>
 __device__ __forceinline__ SeqWork work_of(const AttnParams &p, const Seq &s) {
+  constexpr int kRows = L::kRows, kTile = L::kTile;
   SeqWork w{0, 0, 0, 0};
   const int64_t rows = static_cast<int64_t>(s.fresh) * p.group;
   if (rows == 0 || rows > p.max_rows) return w;
@@ -191,6 +224,7 @@ struct Place {
 };
 
 // This CTA's place in the line.  Thread t sums the sequences [t m, t m + m).
+template <class L>
 __device__ __forceinline__ bool find_place(const AttnParams &p, Place &out) {
   __shared__ int64_t warp_sum[kThreads / 32];
   __shared__ Place found;
@@ -198,7 +232,7 @@ __device__ __forceinline__ bool find_place(const AttnParams &p, Place &out) {
   const int m = (p.batch + kThreads - 1) / kThreads;
   const int lo = min(tid * m, p.batch), hi = min(lo + m, p.batch);
   int64_t sum = 0;
-  for (int i = lo; i < hi; ++i) sum += work_of(p, load_seq(p, i, blockIdx.x == 0)).units;
+  for (int i = lo; i < hi; ++i) sum += work_of<L>(p, load_seq(p, i, blockIdx.x == 0)).units;
   int64_t scan = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -219,7 +253,7 @@ __device__ __forceinline__ bool find_place(const AttnParams &p, Place &out) {
   if (before <= at && at < before + sum) {
     int i = lo;
     for (; i < hi - 1; ++i) {
-      const int64_t u = work_of(p, load_seq(p, i, false)).units;
+      const int64_t u = work_of<L>(p, load_seq(p, i, false)).units;
       if (at < before + u) break;
       before += u;
     }
@@ -233,15 +267,17 @@ __device__ __forceinline__ bool find_place(const AttnParams &p, Place &out) {
 // ---------------------------------------------------------------------------
 // Loading warp
 // ---------------------------------------------------------------------------
-template <int D, bool Q8>
-__device__ void load_units(const AttnParams &p, const Place &place, uint8_t *stages, uint64_t *full, uint64_t *empty) {
-  using L = Layout<D, Q8>;
+template <int D, bool Q8, int NB>
+__device__ __forceinline__ void load_units(const AttnParams &p, const Place &place, uint8_t *stages, uint64_t *full,
+                                           uint64_t *empty) {
+  using L = Layout<D, Q8, NB>;
+  constexpr int kTile = L::kTile, kRows = L::kRows, KT = kTile / 32;  // tokens of a lane
   const int lane = threadIdx.x & 31;
   const int64_t first = place.run * blockIdx.x;
   const int count = static_cast<int>(min(place.run, place.total - first));
   int i = place.seq;
   Seq s = load_seq(p, i, false);
-  SeqWork w = work_of(p, s);
+  SeqWork w = work_of<L>(p, s);
   int64_t begin = place.start;  // units before sequence i
   int rt_tile = static_cast<int>(place.within % w.tiles);
   int64_t rest = place.within / w.tiles;
@@ -249,28 +285,25 @@ __device__ void load_units(const AttnParams &p, const Place &place, uint8_t *sta
   int head = static_cast<int>(rest / w.row_tiles);
   Span v = span_of(p, s, 0, s.fresh);
 
-  // page ids of two tokens per lane, looked up one unit ahead
-  int base, cnt, page[2];
+  // page ids of the lane's tokens, looked up one unit ahead
+  constexpr int kUnused = -0x7fffffff, kNoEntry = -0x7ffffffe;  // not a token of the tile; no such entry
+  int base, cnt, page[KT];
   auto look_up = [&]() {
     const bool in_head = rt_tile < w.head_tiles;
     const int t = in_head ? rt_tile : rt_tile - w.head_tiles;
     base = (in_head ? 0 : v.low) + t * kTile;
     cnt = min(kTile, (in_head ? v.head : v.end) - base);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < KT; ++k) {
       const int t2 = lane + 32 * k;
-      page[k] = -1;
+      page[k] = kUnused;
       if (t2 < cnt) {
         const int64_t e = static_cast<int64_t>(s.e0) + p.by_page.div(base + t2);
-        if (e >= 0 && e < p.indices_cap) {
+        // (the id is not looked at here, so that the load stays in flight)
+        if (e >= 0 && e < p.indices_cap)
           page[k] = __ldg(p.kv_indices + e);
-          if (page[k] < 0 || page[k] >= p.num_pages) {
-            page[k] = -1;
-            raise_deverr(p.error_word, YL_DEVERR_PAGE_RANGE);
-          }
-        } else {
-          raise_deverr(p.error_word, YL_DEVERR_INDICES_CAP);
-        }
+        else
+          page[k] = kNoEntry;
       }
     }
   };
@@ -285,13 +318,14 @@ __device__ void load_units(const AttnParams &p, const Place &place, uint8_t *sta
     const Seq us = s;
     const SeqWork uw = w;
     const int64_t seg = begin + (static_cast<int64_t>(head) * w.row_tiles + rt) * w.tiles;  // its first unit in the line
-    int64_t off[2];
-    uint32_t valid[2];
-    int64_t sc[2];
+    int64_t off[KT], sc[KT];
+    uint32_t valid[KT];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < KT; ++k) {
       const int t2 = lane + 32 * k;
-      const bool ok = page[k] >= 0;
+      const bool ok = page[k] >= 0 && page[k] < p.num_pages;
+      if (!ok && page[k] != kUnused)
+        raise_deverr(p.error_word, page[k] == kNoEntry ? YL_DEVERR_INDICES_CAP : YL_DEVERR_PAGE_RANGE);
       const int pos = u_base + t2;
       const int slot = pos - static_cast<int>(p.by_page.div(max(pos, 0))) * p.page_size;
       off[k] = ok ? static_cast<int64_t>(page[k]) * p.page_stride + static_cast<int64_t>(slot) * p.slot_stride +
@@ -311,7 +345,7 @@ __device__ void load_units(const AttnParams &p, const Place &place, uint8_t *sta
             begin += w.units;
             do {  // ends: count units remain in the line
               s = load_seq(p, ++i, false);
-              w = work_of(p, s);
+              w = work_of<L>(p, s);
             } while (w.units == 0 && i + 1 < p.batch);
             v = span_of(p, s, 0, s.fresh);
           }
@@ -325,19 +359,19 @@ __device__ void load_units(const AttnParams &p, const Place &place, uint8_t *sta
     }
     constexpr int kRowsPer = 32 / L::kChunks;  // rows of one copy instruction
     const int c = lane % L::kChunks;
-#pragma unroll 4
+#pragma unroll
     for (int j = 0; j < kTile / kRowsPer; ++j) {
       const int r = j * kRowsPer + lane / L::kChunks;
-      const int half = j * kRowsPer / 32;
-      const int64_t o = __shfl_sync(0xffffffffu, half ? off[1] : off[0], r & 31) + c * 16;
-      const bool ok = ((half ? valid[1] : valid[0]) >> (r & 31)) & 1u;
+      const int k = j * kRowsPer / 32;
+      const int64_t o = __shfl_sync(0xffffffffu, off[k], r & 31) + c * 16;
+      const bool ok = (valid[k] >> (r & 31)) & 1u;
       const int at = chunk_at<D, Q8>(r, c);
       cp_async16(sk + at, p.kv[0] + o, ok);
       cp_async16(sv + at, p.kv[1] + o, ok);
     }
     if (Q8) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < KT; ++k) {
         const bool ok = (valid[k] >> lane) & 1u;
         cp_async4(ss + (lane + 32 * k) * 4, p.scale[0] + sc[k], ok);
         cp_async4(ss + kTile * 4 + (lane + 32 * k) * 4, p.scale[1] + sc[k], ok);
@@ -362,8 +396,8 @@ __device__ void load_units(const AttnParams &p, const Place &place, uint8_t *sta
     cp_async_arrive(smem_addr(full + stage));
     if (lane == 0) {
       UnitInfo info;
-      info.valid[0] = valid[0];
-      info.valid[1] = valid[1];
+#pragma unroll
+      for (int k = 0; k < KT; ++k) info.valid[k] = valid[k];
       info.base = u_base;
       info.pos0 = us.total - us.fresh;
       info.row0 = u_rt * kRows;
@@ -379,7 +413,7 @@ __device__ void load_units(const AttnParams &p, const Place &place, uint8_t *sta
       if (us.fresh > 1 && !all) flags |= kRagged;
       info.flags = flags;
       info.part = static_cast<int>(2 * blockIdx.x + (seg >= first ? 1 : 0));
-      *reinterpret_cast<UnitInfo *>(st + 2 * L::kKV + L::kQ + L::kScales) = info;
+      *reinterpret_cast<UnitInfo *>(st + L::kInfo) = info;
       mbar_arrive(full + stage);
       // where the parts of a result lie that began in an earlier CTA
       if (u == 0) {
@@ -403,20 +437,25 @@ __device__ void load_units(const AttnParams &p, const Place &place, uint8_t *sta
 // ---------------------------------------------------------------------------
 // Computing warps
 // ---------------------------------------------------------------------------
-template <typename T, int D, bool Q8>
-__device__ void compute_units(const AttnParams &p, const Place &place, uint8_t *stages, uint64_t *full,
-                              uint64_t *empty, uint64_t *joined, float *merge) {
-  using L = Layout<D, Q8>;
+template <typename T, int D, bool Q8, int NB>
+__device__ __forceinline__ void compute_units(const AttnParams &p, const Place &place, uint8_t *stages, uint64_t *full,
+                                              uint64_t *empty, uint64_t *joined, float *merge) {
+  using L = Layout<D, Q8, NB>;
   constexpr bool BF = std::is_same<T, Bf16>::value && !Q8;  // type of the matrix instructions
-  constexpr int KS = D / 16;                                // k-steps of q.k
-  constexpr int NT = D / 8;                                 // n-tiles of p.v
+  constexpr int KS = D / 16;                                // k-steps of k.q
+  constexpr int MT = L::kTokens / 16;                       // token tiles of this warp
+  constexpr int DT = D / 16;                                // tiles of the head dimension
+  constexpr int W = D >= 128 ? 16 : 8;                      // codes of V that a lane takes at once
+  constexpr int kTile = L::kTile, kRows = L::kRows;
   constexpr float kLift = BF ? 0.f : 15.f;                  // weights are kept times 2^kLift
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = lane >> 2, c = lane & 3;
+  const int t0 = warp * L::kTokens;
   const int64_t first = place.run * blockIdx.x;
   const int count = static_cast<int>(min(place.run, place.total - first));
-  uint32_t qf[KS][4];
-  float acc[NT][4], m[2], l[2], coef[2], vref = 0.f;
+  uint32_t qf[KS][NB][2];
+  // columns of a fragment: query rows 8 b + 2 c and 8 b + 2 c + 1
+  float acc[DT][NB][4], m[NB][2], l[NB][2], coef[NB][2], vref = 0.f;
   int stage = 0;
   uint32_t phase = 0, join_phase = 0;
   for (int u = 0; u < count; ++u) {
@@ -426,231 +465,237 @@ __device__ void compute_units(const AttnParams &p, const Place &place, uint8_t *
       if (lane == 0) raise_deverr(p.error_word, YL_DEVERR_TIMEOUT);
       return;
     }
-    const UnitInfo *info = reinterpret_cast<const UnitInfo *>(st + 2 * L::kKV + L::kQ + L::kScales);
+    const UnitInfo *info = reinterpret_cast<const UnitInfo *>(st + L::kInfo);
     const int flags = info->flags;
     if (flags & kFirst) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int b = 0; b < NB; ++b) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][b][j] = 0.f;
+        m[b][0] = m[b][1] = -INFINITY;
+        l[b][0] = l[b][1] = 0.f;
+        coef[b][0] = coef[b][1] = p.scale_log2;
+        const int row = 8 * b + r;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          // dims of this lane's part of k-step s: 16-bit pools in order; 8-bit
+          // pools 4 neighbouring dims of chunk 4 (s / 4) + c
+          const int d0 = Q8 ? (4 * (s / 4) + c) * 16 + 4 * (s % 4) : s * 16 + 2 * c;
+          const int d1 = Q8 ? d0 + 2 : d0 + 8;
+          auto at = [&](int d) { return sq + row * D * 2 + ((((d >> 3) & ~7) | (((d >> 3) ^ row) & 7)) << 4) + (d & 7) * 2; };
+          qf[s][b][0] = lds32(at(d0));
+          qf[s][b][1] = lds32(at(d1));
+        }
+        if (Q8 && std::is_same<T, Bf16>::value) {
+          // bf16 -> fp16, each row times the power of two that brings its
+          // largest element to [1, 2)
+          uint32_t big = 0;
+#pragma unroll
+          for (int s = 0; s < KS; ++s) big = __vmaxu2(big, __vmaxu2(qf[s][b][0] & 0x7fff7fffu, qf[s][b][1] & 0x7fff7fffu));
+          big = max(big & 0xffffu, big >> 16);
+          big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+          big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+          const int e = min(max(static_cast<int>(big >> 7), 1), 253);  // biased exponent
+          const float to = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+          const float back = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(e) << 23);
+          coef[b][0] = __shfl_sync(0xffffffffu, back, 8 * c);
+          coef[b][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float2 f = Bf16::unpack(qf[s][b][k]);
+              qf[s][b][k] = Fp16::pack(f.x * to, f.y * to);
+            }
+        }
+      }
       vref = 0.f;
-      coef[0] = coef[1] = p.scale_log2;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        // dims of this lane's part of k-step s: 16-bit pools in order; 8-bit
-        // pools 4 neighbouring dims of chunk 4 (s / 4) + c
-        const int d0 = Q8 ? (4 * (s / 4) + c) * 16 + 4 * (s % 4) : s * 16 + 2 * c;
-        const int d1 = Q8 ? d0 + 2 : d0 + 8;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int row = r + (k & 1) * 8, d = k & 2 ? d1 : d0;
-          const int ch = d >> 3;
-          qf[s][k] = lds32(sq + row * D * 2 + (((ch & ~7) | ((ch ^ row) & 7)) << 4) + (d & 7) * 2);
-        }
-      }
-      if (Q8 && std::is_same<T, Bf16>::value) {
-        // bf16 -> fp16, each row times the power of two that brings its largest
-        // element to [1, 2)
-        uint32_t big[2] = {0, 0};
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) big[k & 1] = __vmaxu2(big[k & 1], qf[s][k] & 0x7fff7fffu);
-        float to[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t b = max(big[h] & 0xffffu, big[h] >> 16);
-          b = max(b, __shfl_xor_sync(0xffffffffu, b, 1));
-          b = max(b, __shfl_xor_sync(0xffffffffu, b, 2));
-          const int e = min(max(static_cast<int>(b >> 7), 1), 253);  // biased exponent
-          to[h] = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-          coef[h] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(e) << 23);
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = Bf16::unpack(qf[s][k]);
-            qf[s][k] = Fp16::pack(f.x * to[k & 1], f.y * to[k & 1]);
-          }
-      }
     }
 
-    // scores of this warp's 16 tokens
-    const int t0 = warp * 16;
-    float sc[2][4];
+    // scores of this warp's tokens
+    float sc[MT][NB][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sc[n][j] = 0.f;
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[t][b][j] = 0.f;
     if (Q8) {
 #pragma unroll
       for (int h = 0; h < KS / 4; ++h) {
+        uint4 x[MT][2];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint4 w = lds128(sk + chunk_at<D, true>(t0 + 8 * n + r, 4 * h + c));
-          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mma16816<false>(sc[n], qf[4 * h + i], e4m3_lo(x[i]), e4m3_hi(x[i]));
-        }
-      }
-    } else {
-      const int mi = lane >> 3, row = t0 + (lane & 7) + (mi & 2) * 4;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        uint32_t b[4];
-        ldmatrix4(b, sk + chunk_at<D, false>(row, 2 * s + (mi & 1)));
-        mma16816<BF>(sc[0], qf[s], b[0], b[1]);
-        mma16816<BF>(sc[1], qf[s], b[2], b[3]);
-      }
-    }
-    const uint32_t valid = (info->valid[t0 >> 5] >> (t0 & 31)) & 0xffffu;
-    const int base = info->base + t0;
-    bool seen[2][4];
-    float vs[2][2];
-    float top[2] = {-INFINITY, -INFINITY}, vtop = vref;
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      float ks[2] = {1.f, 1.f};
-      if (Q8) {
-        const uint2 a = lds64(ss + (t0 + 8 * n + 2 * c) * 4), b = lds64(ss + kTile * 4 + (t0 + 8 * n + 2 * c) * 4);
-        ks[0] = __uint_as_float(a.x);
-        ks[1] = __uint_as_float(a.y);
-        vs[n][0] = __uint_as_float(b.x);
-        vs[n][1] = __uint_as_float(b.y);
-        vtop = fmaxf(vtop, fmaxf(vs[n][0], vs[n][1]));
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int tok = 8 * n + 2 * c + (j & 1), h = j >> 1;
-        seen[n][j] = (valid >> tok) & 1u;
-        if (flags & kRagged) {
-          const int row = info->row0 + r + 8 * h;
-          const int t = p.by_group.div(min(row, info->rows - 1));
-          seen[n][j] = seen[n][j] && sees(p, info->pos0 + t, base + tok);
-        }
-        const float x = sc[n][j] * (Q8 ? coef[h] * ks[j & 1] : coef[h]);
-        sc[n][j] = seen[n][j] ? x : -INFINITY;
-        top[h] = fmaxf(top[h], sc[n][j]);
-      }
-    }
-#pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
-      top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
-      if (Q8) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
-    }
-    float keep[2], off[2];
-    const float vkeep = Q8 && vref != vtop ? vref / vtop : 1.f;
-    const float vinv = Q8 && vtop > 0.f ? 1.f / vtop : 0.f;
-    vref = vtop;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float to = fmaxf(m[h], top[h]);
-      const float ref = to == -INFINITY ? 0.f : to;  // nothing seen yet: all weights are 2^-inf = 0
-      keep[h] = fast_exp2(m[h] - ref);
-      off[h] = kLift - ref;
-      m[h] = to;
-      l[h] *= keep[h];
-      keep[h] *= vkeep;
-    }
-    if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        acc[i][0] *= keep[0];
-        acc[i][1] *= keep[0];
-        acc[i][2] *= keep[1];
-        acc[i][3] *= keep[1];
-      }
-    }
-    uint32_t pf[4];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      float e[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        e[j] = fast_exp2(sc[n][j] + off[j >> 1]);
-        l[j >> 1] += e[j];
-        if (Q8) e[j] *= vs[n][j & 1] * vinv;
-      }
-      pf[2 * n] = BF ? Bf16::pack(e[0], e[1]) : Fp16::pack(e[0], e[1]);
-      pf[2 * n + 1] = BF ? Bf16::pack(e[2], e[3]) : Fp16::pack(e[2], e[3]);
-    }
-
-    // weights times values
-    uint32_t bad = 0;  // ragged tiles: this lane's tokens (2c, 2c+1, 2c+8, 2c+9) with an infinity or NaN in V
-    auto multiply = [&](int j, uint32_t b0, uint32_t b1) {
-      if (flags & kRagged) bad |= drop_nonfinite<BF>(b0) | drop_nonfinite<BF>(b1) << 2;
-      mma16816<BF>(acc[j], pf, b0, b1);
-    };
-    if (Q8) {
-      constexpr int NV = D >= 128 ? D / 128 : 1;  // 16-byte chunks of V per token and lane
-      if (D == 64) {
-        uint2 w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int tok = t0 + 2 * c + (k & 1) + (k & 2) * 4;
-          w[k] = lds64(sv + chunk_at<D, true>(tok, r >> 1) + (r & 1) * 8);
+        for (int t = 0; t < MT; ++t) {
+          x[t][0] = lds128(sk + chunk_at<D, true>(t0 + 16 * t + r, 4 * h + c));
+          x[t][1] = lds128(sk + chunk_at<D, true>(t0 + 16 * t + r + 8, 4 * h + c));
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t a = i ? w[0].y : w[0].x, b = i ? w[1].y : w[1].x, e = i ? w[2].y : w[2].x,
-                         f = i ? w[3].y : w[3].x;
-          const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
-          const uint32_t ef0 = __byte_perm(e, f, 0x5140), ef1 = __byte_perm(e, f, 0x7362);
-          multiply(4 * i + 0, e4m3_lo(ab0), e4m3_lo(ef0));
-          multiply(4 * i + 1, e4m3_hi(ab0), e4m3_hi(ef0));
-          multiply(4 * i + 2, e4m3_lo(ab1), e4m3_lo(ef1));
-          multiply(4 * i + 3, e4m3_hi(ab1), e4m3_hi(ef1));
-        }
-      } else {
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int h = 0; h < NV; ++h) {
-          uint32_t w[4][4];
+          for (int t = 0; t < MT; ++t) {
+            const uint32_t w0 = i == 0 ? x[t][0].x : i == 1 ? x[t][0].y : i == 2 ? x[t][0].z : x[t][0].w;
+            const uint32_t w1 = i == 0 ? x[t][1].x : i == 1 ? x[t][1].y : i == 2 ? x[t][1].z : x[t][1].w;
+            const uint32_t a[4] = {e4m3_lo(w0), e4m3_lo(w1), e4m3_hi(w0), e4m3_hi(w1)};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int tok = t0 + 2 * c + (k & 1) + (k & 2) * 4;
-            const uint4 x = lds128(sv + chunk_at<D, true>(tok, r + 8 * h));
-            w[k][0] = x.x;
-            w[k][1] = x.y;
-            w[k][2] = x.z;
-            w[k][3] = x.w;
+            for (int b = 0; b < NB; ++b) mma16816<false>(sc[t][b], a, qf[4 * h + i][b][0], qf[4 * h + i][b][1]);
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t ab0 = __byte_perm(w[0][i], w[1][i], 0x5140), ab1 = __byte_perm(w[0][i], w[1][i], 0x7362);
-            const uint32_t ef0 = __byte_perm(w[2][i], w[3][i], 0x5140), ef1 = __byte_perm(w[2][i], w[3][i], 0x7362);
-            multiply(16 * h + 4 * i + 0, e4m3_lo(ab0), e4m3_lo(ef0));
-            multiply(16 * h + 4 * i + 1, e4m3_hi(ab0), e4m3_hi(ef0));
-            multiply(16 * h + 4 * i + 2, e4m3_lo(ab1), e4m3_lo(ef1));
-            multiply(16 * h + 4 * i + 3, e4m3_hi(ab1), e4m3_hi(ef1));
-          }
-        }
       }
     } else {
       const int mi = lane >> 3, row = t0 + (lane & 7) + (mi & 1) * 8;
 #pragma unroll
-      for (int j = 0; j < NT; j += 2) {
-        uint32_t b[4];
-        ldmatrix4_trans(b, sv + chunk_at<D, false>(row, j + (mi >> 1)));
-        multiply(j, b[0], b[1]);
-        multiply(j + 1, b[2], b[3]);
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          uint32_t a[4];
+          ldmatrix4(a, sk + chunk_at<D, false>(row + 16 * t, 2 * s + (mi >> 1)));
+#pragma unroll
+          for (int b = 0; b < NB; ++b) mma16816<BF>(sc[t][b], a, qf[s][b][0], qf[s][b][1]);
+        }
+    }
+    // bit i: token t0 + i of the tile
+    const uint32_t valid = (info->valid[t0 >> 5] >> (t0 & 31)) & (L::kTokens == 32 ? 0xffffffffu : 0xffffu);
+    float vs[MT][2], vtop = vref;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int tok = t0 + 16 * t + r + 8 * k;
+        const float ks = Q8 ? __uint_as_float(lds32(ss + tok * 4)) : 1.f;
+        vs[t][k] = Q8 ? __uint_as_float(lds32(ss + (kTile + tok) * 4)) : 1.f;
+        if (Q8) vtop = fmaxf(vtop, vs[t][k]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) sc[t][b][2 * k + j] *= Q8 ? coef[b][j] * ks : coef[b][j];
       }
+    uint32_t ghosts = 0;  // tokens whose V had an infinity or NaN, zeroed in the stage
+    if (valid != (L::kTokens == 32 ? 0xffffffffu : 0xffffu)) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (!((valid >> (16 * t + r + 4 * (j & 2))) & 1u)) sc[t][b][j] = -INFINITY;
     }
     if (flags & kRagged) {
-      // bits of the lanes that hold the same tokens' other dims
+      ghosts = clean_values<D, Q8, BF, L::kTokens>(sv, t0);
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, d);
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int j = 0; j < 2; ++j) {
+          const int pos = info->pos0 + static_cast<int>(p.by_group.div(min(info->row0 + 8 * b + 2 * c + j, info->rows - 1)));
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (seen[n][j] && (bad >> (2 * n + (j & 1)) & 1u)) l[j >> 1] = NAN;
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int tok = 16 * t + r + 8 * k;
+              if (!sees(p, pos, info->base + t0 + tok))
+                sc[t][b][2 * k + j] = -INFINITY;
+              else if ((ghosts >> tok) & 1u)
+                sc[t][b][2 * k + j] = NAN;
+            }
+        }
+    }
+    float keep[NB][2];
+    bool changed = false;
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1)
+      if (Q8) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
+    const float vkeep = Q8 && vref != vtop ? vref / vtop : 1.f;
+    const float vinv = Q8 && vtop > 0.f ? 1.f / vtop : 0.f;
+    vref = vtop;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float top = fmaxf(sc[0][b][j], sc[0][b][2 + j]);
+#pragma unroll
+        for (int t = 1; t < MT; ++t) top = fmaxf(top, fmaxf(sc[t][b][j], sc[t][b][2 + j]));
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        top = fmaxf(m[b][j], top);
+        const float ref = top == -INFINITY ? 0.f : top;  // nothing seen yet: all weights are 2^-inf = 0
+        const float k = fast_exp2(m[b][j] - ref);
+        m[b][j] = top;
+        l[b][j] *= k;
+        keep[b][j] = k * vkeep;
+        changed |= keep[b][j] != 1.f;
+        const float off = kLift - ref;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          sc[t][b][j] = fast_exp2(sc[t][b][j] + off);
+          sc[t][b][2 + j] = fast_exp2(sc[t][b][2 + j] + off);
+          l[b][j] += sc[t][b][j] + sc[t][b][2 + j];
+        }
+      }
+    if (__any_sync(0xffffffffu, changed)) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][b][j] *= keep[b][j & 1];
+    }
+    uint32_t pf[MT][NB][2];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float w = Q8 ? vs[t][k] * vinv : 1.f;
+          const float x = sc[t][b][2 * k] * w, y = sc[t][b][2 * k + 1] * w;
+          pf[t][b][k] = turn(BF ? Bf16::pack(x, y) : Fp16::pack(x, y));
+        }
+
+    // values times weights
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      if (Q8) {
+#pragma unroll
+        for (int h = 0; h < (D == 256 ? 2 : 1); ++h) {
+          uint32_t w[4][W / 4];  // codes of tokens 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int tok = t0 + 16 * t + 2 * c + (k & 1) + (k & 2) * 4;
+            if (W == 16) {
+              const uint4 x = lds128(sv + chunk_at<D, true>(tok, r + 8 * h));
+              w[k][0] = x.x;
+              w[k][1] = x.y;
+              w[k][W / 4 - 2] = x.z;
+              w[k][W / 4 - 1] = x.w;
+            } else {
+              const uint2 x = lds64(sv + chunk_at<D, true>(tok, r >> 1) + (r & 1) * 8);
+              w[k][0] = x.x;
+              w[k][1] = x.y;
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < W / 4; ++g)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t lo = __byte_perm(w[0][g], w[1][g], i ? 0x7362 : 0x5140);
+              const uint32_t hi = __byte_perm(w[2][g], w[3][g], i ? 0x7362 : 0x5140);
+              const uint32_t a[4] = {e4m3_lo(lo), e4m3_hi(lo), e4m3_lo(hi), e4m3_hi(hi)};
+#pragma unroll
+              for (int b = 0; b < NB; ++b) mma16816<false>(acc[8 * h + 2 * g + i][b], a, pf[t][b][0], pf[t][b][1]);
+            }
+        }
+      } else {
+        const int mi = lane >> 3, row = t0 + 16 * t + (lane & 7) + (mi >> 1) * 8;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          uint32_t a[4];
+          ldmatrix4_trans(a, sv + chunk_at<D, false>(row, 2 * i + (mi & 1)));
+#pragma unroll
+          for (int b = 0; b < NB; ++b) mma16816<BF>(acc[i][b], a, pf[t][b][0], pf[t][b][1]);
+        }
+      }
     }
 
-    const bool last = flags & kLast;
     const int head = info->head, row0 = info->row0, rows = info->rows, part = info->part;
     const int64_t q0 = info->q0;
     __syncwarp();
@@ -659,21 +704,22 @@ __device__ void compute_units(const AttnParams &p, const Place &place, uint8_t *
       stage = 0;
       phase ^= 1;
     }
-    if (!last) continue;
+    if (!(flags & kLast)) continue;
 
     // Join the four warps: 2 and 3 into 0 and 1, then 1 into 0.
 #pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
-      l[1] += __shfl_xor_sync(0xffffffffu, l[1], d);
-    }
-    if (Q8) {
+    for (int b = 0; b < NB; ++b) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] *= vref;
+        for (int d = 4; d < 32; d <<= 1) l[b][j] += __shfl_xor_sync(0xffffffffu, l[b][j], d);
+      if (Q8) {
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][b][j] *= vref;
+      }
     }
-    float *stats = merge + 2 * kRows * D;  // [2][2][16]: maximum and sum of a giving warp's rows
     auto meet = [&]() -> bool {
       __syncwarp();
       if (lane == 0) mbar_arrive(joined);
@@ -683,34 +729,41 @@ __device__ void compute_units(const AttnParams &p, const Place &place, uint8_t *
       return ok;
     };
     auto give = [&](int to) {
-      float *a = merge + to * kRows * D, *b = stats + to * 2 * kRows;
+      float *a = merge + to * (kRows * D + 2 * kRows), *s = a + kRows * D;
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int b = 0; b < NB; ++b) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a[(i * 4 + j) * 32 + lane] = acc[i][j];
-      if (c == 0) {
-        b[r] = m[0];
-        b[r + 8] = m[1];
-        b[kRows + r] = l[0];
-        b[kRows + r + 8] = l[1];
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) a[((i * NB + b) * 4 + j) * 32 + lane] = acc[i][b][j];
+        if (r == 0) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[8 * b + 2 * c + j] = m[b][j];
+            s[kRows + 8 * b + 2 * c + j] = l[b][j];
+          }
+        }
       }
     };
     auto take = [&](int from) {
-      const float *a = merge + from * kRows * D, *b = stats + from * 2 * kRows;
-      float mine[2], theirs[2];
+      const float *a = merge + from * (kRows * D + 2 * kRows), *s = a + kRows * D;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float om = b[r + 8 * h], to = fmaxf(m[h], om), ref = to == -INFINITY ? 0.f : to;
-        mine[h] = fast_exp2(m[h] - ref);
-        theirs[h] = fast_exp2(om - ref);
-        m[h] = to;
-        l[h] = l[h] * mine[h] + b[kRows + r + 8 * h] * theirs[h];
+      for (int b = 0; b < NB; ++b) {
+        float mine[2], theirs[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float om = s[8 * b + 2 * c + j], top = fmaxf(m[b][j], om), ref = top == -INFINITY ? 0.f : top;
+          mine[j] = fast_exp2(m[b][j] - ref);
+          theirs[j] = fast_exp2(om - ref);
+          m[b][j] = top;
+          l[b][j] = l[b][j] * mine[j] + s[kRows + 8 * b + 2 * c + j] * theirs[j];
+        }
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[i][b][j] = acc[i][b][j] * mine[j & 1] + a[((i * NB + b) * 4 + j) * 32 + lane] * theirs[j & 1];
       }
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = acc[i][j] * mine[j >> 1] + a[(i * 4 + j) * 32 + lane] * theirs[j >> 1];
     };
     if (warp >= 2) give(warp - 2);
     if (!meet()) return;
@@ -720,81 +773,66 @@ __device__ void compute_units(const AttnParams &p, const Place &place, uint8_t *
     if (!meet()) return;
     if (warp == 0) take(0);
     if (!meet()) return;  // before the next give
-    if (warp == 0) {
-      if (flags & kWhole) {
+    if (warp != 0) continue;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = row0 + r + 8 * h;
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int col = 8 * b + 2 * c + j, row = row0 + col;
+        if (row >= rows) continue;
+        if (flags & kWhole) {
           const int t = p.by_group.div(row), g = row - t * p.group;
-          if (row >= rows || q0 + t >= p.num_tokens) continue;
+          if (q0 + t >= p.num_tokens) continue;
           char *out = p.o + (q0 + t) * p.o_row_stride + (static_cast<int64_t>(head) * p.group + g) * p.o_head_stride;
-          const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
+          const float inv = l[b][j] == 0.f ? 0.f : 1.f / l[b][j];
           if (Q8) {
-            // lane c of a row holds dims (2c + k) W .. + W of each W * 8 dims, W neighbouring n-tiles
-            constexpr int W = D >= 128 ? 16 : 8;
+            // dims r W .. + W of each 8 W
 #pragma unroll
-            for (int b = 0; b < NT / W; ++b)
+            for (int i = 0; i < DT; i += 4) {
+              uint32_t w[4];
 #pragma unroll
-              for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int i = 0; i < W; i += 8) {
-                  uint32_t w[4];
-#pragma unroll
-                  for (int x = 0; x < 4; ++x)
-                    w[x] = T::pack(acc[b * W + i + 2 * x][2 * h + k] * inv, acc[b * W + i + 2 * x + 1][2 * h + k] * inv);
-                  *reinterpret_cast<uint4 *>(out + (b * W * 8 + (2 * c + k) * W + i) * 2) =
-                      make_uint4(w[0], w[1], w[2], w[3]);
-                }
-          } else {
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-              *reinterpret_cast<uint32_t *>(out + (i * 8 + 2 * c) * 2) =
-                  T::pack(acc[i][2 * h] * inv, acc[i][2 * h + 1] * inv);
-          }
-        }
-      } else {
-        // in the order of the registers: the joining kernel knows it
-        float *a = p.partials + static_cast<int64_t>(part) * (kRows * D + 2 * kRows), *b = a + kRows * D;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = r + 8 * h;
-          if (row0 + row >= rows) continue;
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            float2 *at;
-            float x, y;
-            if (Q8) {
-              constexpr int W = D >= 128 ? 16 : 8;
-              // pairs of neighbouring n-tiles are neighbouring dims
-              const int k = i & 1, j = i & ~1;
-              at = reinterpret_cast<float2 *>(a + row * D + (j / W) * W * 8 + (2 * c + k) * W + j % W);
-              x = acc[j][2 * h + k];
-              y = acc[j + 1][2 * h + k];
-            } else {
-              at = reinterpret_cast<float2 *>(a + row * D + i * 8 + 2 * c);
-              x = acc[i][2 * h];
-              y = acc[i][2 * h + 1];
+              for (int x = 0; x < 4; ++x) w[x] = T::pack(acc[i + x][b][j] * inv, acc[i + x][b][2 + j] * inv);
+              *reinterpret_cast<uint4 *>(out + ((2 * i / W) * W * 8 + r * W + 2 * i % W) * 2) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
             }
-            *at = make_float2(x, y);
+          } else {
+            // dims r and r + 8 of each 16: a neighbour's dim beside this lane's
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+              const float x = acc[i][b][j] * inv, y = acc[i][b][2 + j] * inv;
+              *reinterpret_cast<uint16_t *>(out + (16 * i + r) * 2) = static_cast<uint16_t>(T::pack(x, 0.f));
+              *reinterpret_cast<uint16_t *>(out + (16 * i + 8 + r) * 2) = static_cast<uint16_t>(T::pack(y, 0.f));
+            }
           }
-          if (c == 0) {
-            b[row] = m[h];
-            b[kRows + row] = l[h];
+        } else {
+          float *a = p.partials + static_cast<int64_t>(part) * (kRows * D + 2 * kRows), *s = a + kRows * D;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) {
+            if (Q8) {
+              *reinterpret_cast<float2 *>(a + col * D + (2 * i / W) * W * 8 + r * W + 2 * i % W) =
+                  make_float2(acc[i][b][j], acc[i][b][2 + j]);
+            } else {
+              a[col * D + 16 * i + r] = acc[i][b][j];
+              a[col * D + 16 * i + 8 + r] = acc[i][b][2 + j];
+            }
+          }
+          if (r == 0) {
+            s[col] = m[b][j];
+            s[kRows + col] = l[b][j];
           }
         }
       }
-    }
   }
 }
 
-template <typename T, int D, bool Q8>
-__global__ void __launch_bounds__(kThreads, Layout<D, Q8>::kCtas) decode_kernel(const __grid_constant__ AttnParams p) {
-  using L = Layout<D, Q8>;
+template <typename T, int D, bool Q8, int NB>
+__global__ void __launch_bounds__(kThreads, Layout<D, Q8, NB>::kCtas)
+    decode_kernel(const __grid_constant__ AttnParams p) {
+  using L = Layout<D, Q8, NB>;
   extern __shared__ uint8_t raw[];
-  uint8_t *smem = raw + ((128 - (smem_addr(raw) & 127)) & 127);
-  uint8_t *stages = smem;
-  float *merge = reinterpret_cast<float *>(smem + L::kStages * L::kStage);
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::kStages * L::kStage + L::kMerge + 256);
+  uint8_t *stages = raw + ((128 - (smem_addr(raw) & 127)) & 127);
+  float *merge = reinterpret_cast<float *>(stages + L::kStages * L::kStage);
+  uint64_t *full = reinterpret_cast<uint64_t *>(stages + L::kStages * L::kStage + L::kMerge);
   uint64_t *empty = full + L::kStages, *joined = empty + L::kStages;
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kStages; ++i) {
@@ -805,16 +843,16 @@ __global__ void __launch_bounds__(kThreads, Layout<D, Q8>::kCtas) decode_kernel(
   }
   pdl_wait();
   Place place;
-  const bool work = find_place(p, place);  // synchronises the block
+  const bool work = find_place<L>(p, place);  // synchronises the block
   pdl_trigger();
   if (!work) {
     if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
   if (threadIdx.x >= kConsumers * 32)
-    load_units<D, Q8>(p, place, stages, full, empty);
+    load_units<D, Q8, NB>(p, place, stages, full, empty);
   else
-    compute_units<T, D, Q8>(p, place, stages, full, empty, joined, merge);
+    compute_units<T, D, Q8, NB>(p, place, stages, full, empty, joined, merge);
 }
 
 // Joins the parts of a result that began in CTA c - 1 and goes on in CTA c (and
@@ -822,9 +860,9 @@ __global__ void __launch_bounds__(kThreads, Layout<D, Q8>::kCtas) decode_kernel(
 // follow.  One block per (c, query row); 32 lanes per part, parts in turn over
 // the warps, then the warps in order.
 constexpr int kJoinWarps = 4;
-template <typename T, int D>
+template <typename T, int D, int NB>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int N = D / 32;
+  constexpr int N = D / 32, kRows = 8 * NB;
   __shared__ float part[kJoinWarps][D + 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x + 1, r = blockIdx.y;
   pdl_wait();
@@ -874,15 +912,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
     *reinterpret_cast<uint32_t *>(out + (i * 32 + 2 * lane) * 2) = T::pack(acc[i] * inv, acc[i + 1] * inv);
 }
 
-// The grid of the decode kernel and the bytes of its parts.
-int decode_ctas(int D, bool q8) {
-  int per_sm = 1;
-  if (D == 64) per_sm = q8 ? Layout<64, true>::kCtas : Layout<64, false>::kCtas;
-  if (D == 128) per_sm = q8 ? Layout<128, true>::kCtas : Layout<128, false>::kCtas;
-  if (D == 256) per_sm = q8 ? Layout<256, true>::kCtas : Layout<256, false>::kCtas;
-  return sm_count() * per_sm;
-}
-
 // Shared memory above 48 KB is asked for once per kernel and device.
 int allow_smem(const void *fn, int bytes) {
   static std::mutex mu;
@@ -900,41 +929,49 @@ int allow_smem(const void *fn, int bytes) {
   return YL_OK;
 }
 
-template <typename T, int D, bool Q8>
-int launch(AttnParams &p, int ctas, int rows, cudaStream_t stream) {
-  int rc = allow_smem(reinterpret_cast<const void *>(decode_kernel<T, D, Q8>), Layout<D, Q8>::kSmem);
-  if (rc != YL_OK) return rc;
-  rc = launch_dependent(decode_kernel<T, D, Q8>, dim3(ctas), dim3(kThreads), Layout<D, Q8>::kSmem, stream,
-                        "yl_paged_attention launch", p);
-  if (rc != YL_OK) return rc;
-  return launch_dependent(join_kernel<T, D>, dim3(ctas - 1, rows), dim3(kJoinWarps * 32), 0,
-                          stream, "yl_paged_attention launch", p);
+template <typename F>
+auto pick(int dtype, int dim, bool q8, int64_t most_rows, F f) {
+  auto rows = [&](auto t, auto d, auto q) {
+    // 8 query rows a unit where no sequence has more, else 16
+    if (most_rows <= 8) return f(t, d, q, std::integral_constant<int, 1>{});
+    return f(t, d, q, std::integral_constant<int, 2>{});
+  };
+  auto kind = [&](auto t, auto d) { return q8 ? rows(t, d, std::true_type{}) : rows(t, d, std::false_type{}); };
+  auto head = [&](auto t) {
+    if (dim == 64) return kind(t, std::integral_constant<int, 64>{});
+    if (dim == 128) return kind(t, std::integral_constant<int, 128>{});
+    return kind(t, std::integral_constant<int, 256>{});
+  };
+  return dtype == YL_DTYPE_BF16 ? head(Bf16{}) : head(Fp16{});
 }
 
 }  // namespace
 
-int64_t decode_workspace(const yl_paged_attention_args *a) {
-  const int64_t ctas = decode_ctas(a->head_dim, a->kv_dtype == YL_KV_E4M3);
-  return ctas * 16 + ctas * 2 * (kRows * a->head_dim + 2 * kRows) * 4;
+int64_t decode_workspace(const yl_paged_attention_args *a, int64_t most_rows) {
+  return pick(a->dtype, a->head_dim, a->kv_dtype == YL_KV_E4M3, most_rows, [](auto, auto d, auto q, auto b) {
+    using L = Layout<decltype(d)::value, decltype(q)::value, decltype(b)::value>;
+    const int64_t ctas = static_cast<int64_t>(sm_count()) * L::kCtas;
+    return ctas * 16 + ctas * 2 * (L::kRows * decltype(d)::value + 2 * L::kRows) * 4;
+  });
 }
 
 int launch_decode(AttnParams &p, const yl_paged_attention_args *a, int64_t most_rows, cudaStream_t stream) {
-  const bool q8 = a->kv_dtype == YL_KV_E4M3;
-  const int ctas = decode_ctas(a->head_dim, q8);
-  const int rows = static_cast<int>(std::min<int64_t>(most_rows, kRows));
-  p.meta = static_cast<int4 *>(a->workspace);
-  p.partials = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + ctas * 16);
-  auto go = [&](auto t, auto d) {
+  return pick(a->dtype, a->head_dim, a->kv_dtype == YL_KV_E4M3, most_rows, [&](auto t, auto d, auto q, auto b) {
     using T = decltype(t);
-    constexpr int D = decltype(d)::value;
-    return q8 ? launch<T, D, true>(p, ctas, rows, stream) : launch<T, D, false>(p, ctas, rows, stream);
-  };
-  auto dim = [&](auto t) {
-    if (a->head_dim == 64) return go(t, std::integral_constant<int, 64>{});
-    if (a->head_dim == 128) return go(t, std::integral_constant<int, 128>{});
-    return go(t, std::integral_constant<int, 256>{});
-  };
-  return a->dtype == YL_DTYPE_BF16 ? dim(Bf16{}) : dim(Fp16{});
+    constexpr int D = decltype(d)::value, NB = decltype(b)::value;
+    constexpr bool Q8 = decltype(q)::value;
+    using L = Layout<D, Q8, NB>;
+    const int ctas = sm_count() * L::kCtas;
+    p.meta = static_cast<int4 *>(a->workspace);
+    p.partials = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + static_cast<int64_t>(ctas) * 16);
+    int rc = allow_smem(reinterpret_cast<const void *>(decode_kernel<T, D, Q8, NB>), L::kSmem);
+    if (rc != YL_OK) return rc;
+    rc = launch_dependent(decode_kernel<T, D, Q8, NB>, dim3(ctas), dim3(kThreads), L::kSmem, stream,
+                          "yl_paged_attention launch", p);
+    if (rc != YL_OK) return rc;
+    return launch_dependent(join_kernel<T, D, NB>, dim3(ctas - 1, static_cast<unsigned>(std::min<int64_t>(most_rows, L::kRows))),
+                            dim3(kJoinWarps * 32), 0, stream, "yl_paged_attention launch", p);
+  });
 }
 
 }  // namespace ylk

@@ -103,7 +103,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
 
 // The decode kernel: workspace bytes, and its launch for sequences of at most
 // p.max_rows query rows per KV head, none of which has more than most_rows.
-int64_t decode_workspace(const yl_paged_attention_args *a);
+int64_t decode_workspace(const yl_paged_attention_args *a, int64_t most_rows);
 int launch_decode(AttnParams &p, const yl_paged_attention_args *a, int64_t most_rows, cudaStream_t stream);
 
 }  // namespace ylk

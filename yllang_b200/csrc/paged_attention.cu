@@ -95,6 +95,12 @@ __global__ void __launch_bounds__(kSimpleWarps * 32) attend_kernel(const __grid_
   }
 }
 
+// Most query rows per KV head that a sequence of the call can have.
+int64_t most_rows(const yl_paged_attention_args *a) {
+  const int64_t fresh = a->max_new_len > 0 ? std::min<int64_t>(a->max_new_len, a->num_tokens) : a->num_tokens;
+  return fresh * (a->num_q_heads / a->num_kv_heads);
+}
+
 int check_attention(const yl_paged_attention_args *a, bool pointers) {
   if (a == nullptr) return fail(YL_ERR_NULL_ARG, "yl_paged_attention: args is NULL");
   if (a->batch_size < 0) return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: batch_size=%lld < 0", a->batch_size);
@@ -153,7 +159,7 @@ extern "C" int64_t yl_paged_attention_workspace(const yl_paged_attention_args *a
   using namespace ylk;
   clear_last_error();
   const int rc = check_attention(a, false);
-  return rc != YL_OK ? rc : decode_workspace(a);
+  return rc != YL_OK ? rc : decode_workspace(a, most_rows(a));
 }
 
 extern "C" int yl_paged_attention(const yl_paged_attention_args *a, cudaStream_t stream) {
@@ -162,9 +168,10 @@ extern "C" int yl_paged_attention(const yl_paged_attention_args *a, cudaStream_t
   int rc = check_attention(a, true);
   if (rc != YL_OK) return rc;
   if (a->batch_size == 0 || a->num_tokens == 0) return YL_OK;
-  if (a->workspace == nullptr || a->workspace_bytes < decode_workspace(a))
+  const int64_t most = most_rows(a);
+  if (a->workspace == nullptr || a->workspace_bytes < decode_workspace(a, most))
     return fail(a->workspace ? YL_ERR_BAD_SIZE : YL_ERR_NULL_ARG,
-                "yl_paged_attention: workspace must hold %lld bytes", decode_workspace(a));
+                "yl_paged_attention: workspace must hold %lld bytes", decode_workspace(a, most));
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15u)
     return fail(YL_ERR_ALIGNMENT, "yl_paged_attention: workspace must be 16-byte aligned");
   AttnParams p;
@@ -202,8 +209,6 @@ extern "C" int yl_paged_attention(const yl_paged_attention_args *a, cudaStream_t
   p.by_group = FastDiv(static_cast<uint32_t>(p.group));
   p.scale_log2 = a->sm_scale * 1.44269504088896f;
   p.max_rows = kDecodeRows;
-  // most query rows per KV head that a sequence can have
-  const int64_t most = (a->max_new_len > 0 ? std::min<int64_t>(a->max_new_len, a->num_tokens) : a->num_tokens) * p.group;
   rc = launch_decode(p, a, most, stream);
   if (rc != YL_OK || most <= kDecodeRows) return rc;
   const dim3 grid(static_cast<unsigned>(a->num_tokens), static_cast<unsigned>(a->num_kv_heads));
