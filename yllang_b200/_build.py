@@ -27,7 +27,8 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libyl_kvpath.so")
 
 CUDA_SOURCES = ["common.cu", "kv_store.cu", "index_build.cu", "kv_step.cu", "gather.cu", "qkv_store.cu",
-                "page_alloc.cu", "ranges.cu", "quant_store.cu", "paged_attention.cu"]
+                "page_alloc.cu", "ranges.cu", "quant_store.cu", "paged_attention.cu",
+                "attend_decode.cu", "attend_prefill.cu"]
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

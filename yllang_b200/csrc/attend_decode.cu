@@ -38,9 +38,6 @@
 
 #include <algorithm>
 #include <cstdint>
-#include <map>
-#include <mutex>
-#include <tuple>
 
 #include "attend_device.cuh"
 #include "tma.cuh"
@@ -910,23 +907,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
 #pragma unroll
   for (int i = 0; i < N; i += 2)
     *reinterpret_cast<uint32_t *>(out + (i * 32 + 2 * lane) * 2) = T::pack(acc[i] * inv, acc[i + 1] * inv);
-}
-
-// Shared memory above 48 KB is asked for once per kernel and device.
-int allow_smem(const void *fn, int bytes) {
-  static std::mutex mu;
-  static std::map<std::pair<int, const void *>, int> done;
-  std::lock_guard<std::mutex> lock(mu);
-  int &have = done[std::make_pair(current_device(), fn)];
-  if (have >= bytes) return YL_OK;
-  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    set_last_error(std::string("yl_paged_attention: shared memory: ") + cudaGetErrorString(e));
-    return YL_ERR_CUDA;
-  }
-  have = bytes;
-  return YL_OK;
 }
 
 template <typename F>

@@ -101,9 +101,15 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// Lets a kernel have `bytes` of dynamic shared memory on the current device
+// (asked for once per kernel and device); a yl_status.
+int allow_smem(const void *fn, int bytes);
+
 // The decode kernel: workspace bytes, and its launch for sequences of at most
 // p.max_rows query rows per KV head, none of which has more than most_rows.
 int64_t decode_workspace(const yl_paged_attention_args *a, int64_t most_rows);
 int launch_decode(AttnParams &p, const yl_paged_attention_args *a, int64_t most_rows, cudaStream_t stream);
+// The prefill kernel, for sequences of more than p.max_rows rows.
+int launch_prefill(AttnParams &p, const yl_paged_attention_args *a, cudaStream_t stream);
 
 }  // namespace ylk

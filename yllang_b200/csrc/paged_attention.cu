@@ -1,99 +1,20 @@
-// Paged attention over a 16-bit or an 8-bit pool, causal from each sequence's
-// end, with an optional sliding window and first tokens that stay visible.
-//
-// One warp per (new token, query head): the lanes split the head dimension and
-// the warp walks the visible positions with a running maximum and sum.
+// yl_paged_attention: argument checks, and which kernel takes which sequence of
+// the batch (attend_decode.cu, attend_prefill.cu).
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <map>
+#include <mutex>
 
 #include "attend_device.cuh"
 
 namespace ylk {
 namespace {
 
-constexpr int kSimpleWarps = 4;
-constexpr int kDecodeRows = 64;  // query rows per KV head up to which a sequence is the decode kernel's
-
-template <typename T, bool Q8, int N>
-__device__ __forceinline__ void load_row(const char *at, float scale, float (&x)[N]) {
-  if (Q8) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint16_t c = *reinterpret_cast<const uint16_t *>(at + i);
-      const float2 f = half2_bits_to_float2(e4m3x2_to_half2(c));
-      x[i] = f.x * scale;
-      x[i + 1] = f.y * scale;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 f = T::unpack(*reinterpret_cast<const uint32_t *>(at + 2 * i));
-      x[i] = f.x;
-      x[i + 1] = f.y;
-    }
-  }
-}
-
-template <typename T, int D, bool Q8>
-__global__ void __launch_bounds__(kSimpleWarps * 32) attend_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int N = D / 32;
-  constexpr int kItem = Q8 ? 1 : 2;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = blockIdx.x;
-  const int kvh = blockIdx.y;
-  pdl_wait();
-  const int i = warp_find(p.batch, row, lane, [&](int s) -> int64_t { return __ldg(p.qo_indptr + s); });
-  const bool report = threadIdx.x == 0 && kvh == 0;
-  const Seq sq = load_seq(p, i, report);
-  if (row < sq.q0 || row >= static_cast<int64_t>(sq.q0) + sq.fresh) return;  // behind the last sequence
-  if (static_cast<int64_t>(sq.fresh) * p.group <= p.max_rows) return;        // the decode kernel's
-  const int64_t e0 = sq.e0;
-  const int pos = max(sq.total - sq.fresh + static_cast<int>(row - sq.q0), -1);
-  const int low = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
-  const int head = min(p.window > 0 ? p.sinks : 0, low);
-  for (int g = threadIdx.x >> 5; g < p.group; g += kSimpleWarps) {
-    const int h = kvh * p.group + g;
-    float q[N], acc[N], m = -INFINITY, l = 0.f;
-    load_row<T, false>(p.q + row * p.q_row_stride + h * p.q_head_stride + lane * N * 2, 1.f, q);
-#pragma unroll
-    for (int d = 0; d < N; ++d) acc[d] = 0.f;
-    for (int s = 0; s < head + (pos + 1 - low); ++s) {
-      const int j = s < head ? s : low + s - head;
-      const int64_t e = e0 + j / p.page_size;
-      if (e < 0 || e >= p.indices_cap) {
-        if (report) raise_deverr(p.error_word, YL_DEVERR_INDICES_CAP);
-        continue;
-      }
-      const int64_t page = __ldg(p.kv_indices + e);
-      if (page < 0 || page >= p.num_pages) {
-        if (report) raise_deverr(p.error_word, YL_DEVERR_PAGE_RANGE);
-        continue;
-      }
-      const int64_t at = page * p.page_stride + (j % p.page_size) * p.slot_stride + kvh * p.head_stride + lane * N * kItem;
-      const int64_t sc = page * p.scale_page_stride + kvh * p.scale_head_stride;
-      float k[N], v[N], dot = 0.f;
-      load_row<T, Q8>(p.kv[0] + at, Q8 ? __ldg(p.scale[0] + sc) : 1.f, k);
-      load_row<T, Q8>(p.kv[1] + at, Q8 ? __ldg(p.scale[1] + sc) : 1.f, v);
-#pragma unroll
-      for (int d = 0; d < N; ++d) dot += q[d] * k[d];
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-      dot *= p.scale_log2;
-      const float m2 = fmaxf(m, dot);
-      const float keep = m2 == -INFINITY ? 1.f : exp2f(m - m2), w = m2 == -INFINITY ? 0.f : exp2f(dot - m2);
-      m = m2;
-      l = l * keep + w;
-#pragma unroll
-      for (int d = 0; d < N; ++d) acc[d] = acc[d] * keep + w * v[d];
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    char *out = p.o + row * p.o_row_stride + h * p.o_head_stride + lane * N * 2;
-#pragma unroll
-    for (int d = 0; d < N; d += 2) *reinterpret_cast<uint32_t *>(out + 2 * d) = T::pack(acc[d] * inv, acc[d + 1] * inv);
-  }
-}
+// Query rows per KV head (new tokens times heads of the group) up to which a
+// sequence is the decode kernel's.
+constexpr int kDecodeRows = 64;
 
 // Most query rows per KV head that a sequence of the call can have.
 int64_t most_rows(const yl_paged_attention_args *a) {
@@ -116,6 +37,8 @@ int check_attention(const yl_paged_attention_args *a, bool pointers) {
   if (a->num_kv_heads < 1 || a->num_q_heads < 1 || a->num_q_heads % a->num_kv_heads != 0)
     return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: num_q_heads=%lld must be a multiple of num_kv_heads=%lld",
                 a->num_q_heads, a->num_kv_heads);
+  if (a->num_tokens * (a->num_q_heads / a->num_kv_heads) >= (1ll << 31))
+    return fail(YL_ERR_UNSUPPORTED, "yl_paged_attention: num_tokens=%lld times the group passes 2^31", a->num_tokens);
   if (a->num_kv_heads > 32767)
     return fail(YL_ERR_UNSUPPORTED, "yl_paged_attention: num_kv_heads=%lld exceeds 32767", a->num_kv_heads);
   if (a->page_size < 1) return fail(YL_ERR_BAD_SIZE, "yl_paged_attention: page_size=%lld < 1", a->page_size);
@@ -153,6 +76,23 @@ int check_attention(const yl_paged_attention_args *a, bool pointers) {
 }
 
 }  // namespace
+
+int allow_smem(const void *fn, int bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void *>, int> done;
+  std::lock_guard<std::mutex> lock(mu);
+  int &have = done[std::make_pair(current_device(), fn)];
+  if (have >= bytes) return YL_OK;
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_last_error(std::string("yl_paged_attention: shared memory: ") + cudaGetErrorString(e));
+    return YL_ERR_CUDA;
+  }
+  have = bytes;
+  return YL_OK;
+}
+
 }  // namespace ylk
 
 extern "C" int64_t yl_paged_attention_workspace(const yl_paged_attention_args *a) {
@@ -211,15 +151,5 @@ extern "C" int yl_paged_attention(const yl_paged_attention_args *a, cudaStream_t
   p.max_rows = kDecodeRows;
   rc = launch_decode(p, a, most, stream);
   if (rc != YL_OK || most <= kDecodeRows) return rc;
-  const dim3 grid(static_cast<unsigned>(a->num_tokens), static_cast<unsigned>(a->num_kv_heads));
-  auto go = [&](auto t, auto q8) {
-    using T = decltype(t);
-    constexpr bool Q8 = decltype(q8)::value;
-    auto fn = a->head_dim == 64 ? attend_kernel<T, 64, Q8> : a->head_dim == 128 ? attend_kernel<T, 128, Q8>
-                                                                               : attend_kernel<T, 256, Q8>;
-    return launch_dependent(fn, grid, dim3(kSimpleWarps * 32), 0, stream, "yl_paged_attention launch", p);
-  };
-  const bool q8 = a->kv_dtype == YL_KV_E4M3;
-  if (a->dtype == YL_DTYPE_BF16) return q8 ? go(Bf16{}, std::true_type{}) : go(Bf16{}, std::false_type{});
-  return q8 ? go(Fp16{}, std::true_type{}) : go(Fp16{}, std::false_type{});
+  return launch_prefill(p, a, stream);
 }
