@@ -63,6 +63,74 @@ PYBIND11_MODULE(_C, m) {
   m.def("QKNormRopeStoreKV", &QKNormRopeStoreKV, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("k_cache"),
         py::arg("v_cache"), py::arg("indices"), py::arg("opts"), py::arg("q_out"));
 
+  // the page arrays are passed one by one, as the Python front end's BatchIndex holds them
+  m.def(
+      "StoreKVCacheQuant",
+      [](const torch::Tensor &k, const torch::Tensor &v, const torch::Tensor &pool_k, const torch::Tensor &pool_v,
+         const torch::Tensor &k_scale, const torch::Tensor &v_scale, const torch::Tensor &kv_indptr,
+         const torch::Tensor &kv_indices, const torch::Tensor &kv_last_page_len, const torch::Tensor &qo_indptr,
+         const std::optional<torch::Tensor> &error_word) {
+        StoreKVCacheQuant(k, v, {pool_k, pool_v, k_scale, v_scale}, {kv_indptr, kv_indices, kv_last_page_len, qo_indptr, {}},
+                          error_word);
+      },
+      py::arg("k"), py::arg("v"), py::arg("pool_k"), py::arg("pool_v"), py::arg("k_scale"), py::arg("v_scale"),
+      py::arg("kv_indptr"), py::arg("kv_indices"), py::arg("kv_last_page_len"), py::arg("qo_indptr"),
+      py::arg("error_word") = py::none(), "quantise a batch's new K/V rows into an 8-bit pool");
+  m.def(
+      "LoadKVCacheQuant",
+      [](const torch::Tensor &pool_k, const torch::Tensor &pool_v, const torch::Tensor &k_scale,
+         const torch::Tensor &v_scale, const torch::Tensor &slots, py::object dtype,
+         const std::optional<std::pair<torch::Tensor, torch::Tensor>> &out, const std::optional<torch::Tensor> &error_word) {
+        return LoadKVCacheQuant({pool_k, pool_v, k_scale, v_scale}, slots, torch::python::detail::py_object_to_dtype(dtype),
+                                out, error_word);
+      },
+      py::arg("pool_k"), py::arg("pool_v"), py::arg("k_scale"), py::arg("v_scale"), py::arg("slots"), py::arg("dtype"),
+      py::arg("out") = py::none(), py::arg("error_word") = py::none(), "rows of an 8-bit pool in bf16 or fp16");
+  const auto attention_options = [](const std::optional<torch::Tensor> &k_scale, const std::optional<torch::Tensor> &v_scale,
+                                    int64_t window, int64_t sinks, std::optional<double> sm_scale, int64_t max_new_len) {
+    PagedAttentionOptions o;
+    o.k_scale = k_scale;
+    o.v_scale = v_scale;
+    o.window = window;
+    o.sinks = sinks;
+    o.sm_scale = sm_scale;
+    o.max_new_len = max_new_len;
+    return o;
+  };
+  m.def(
+      "PagedAttention",
+      [attention_options](const torch::Tensor &q, const torch::Tensor &k_pages, const torch::Tensor &v_pages,
+                          const torch::Tensor &kv_indptr, const torch::Tensor &kv_indices,
+                          const torch::Tensor &kv_last_page_len, const torch::Tensor &qo_indptr,
+                          const std::optional<torch::Tensor> &k_scale, const std::optional<torch::Tensor> &v_scale,
+                          int64_t window, int64_t sinks, std::optional<double> sm_scale, int64_t max_new_len,
+                          const std::optional<torch::Tensor> &out, const std::optional<torch::Tensor> &workspace,
+                          const std::optional<torch::Tensor> &error_word) {
+        auto o = attention_options(k_scale, v_scale, window, sinks, sm_scale, max_new_len);
+        o.out = out;
+        o.workspace = workspace;
+        o.error_word = error_word;
+        return PagedAttention(q, k_pages, v_pages, {kv_indptr, kv_indices, kv_last_page_len, qo_indptr, {}}, o);
+      },
+      py::arg("q"), py::arg("k_pages"), py::arg("v_pages"), py::arg("kv_indptr"), py::arg("kv_indices"),
+      py::arg("kv_last_page_len"), py::arg("qo_indptr"), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(),
+      py::arg("window") = 0, py::arg("sinks") = 0, py::arg("sm_scale") = py::none(), py::arg("max_new_len") = 0,
+      py::arg("out") = py::none(), py::arg("workspace") = py::none(), py::arg("error_word") = py::none(),
+      "attention of a batch's new tokens over the paged pool");
+  m.def(
+      "PagedAttentionWorkspace",
+      [attention_options](const torch::Tensor &q, const torch::Tensor &k_pages, const torch::Tensor &v_pages,
+                          const torch::Tensor &kv_indptr, const torch::Tensor &kv_indices,
+                          const torch::Tensor &kv_last_page_len, const torch::Tensor &qo_indptr,
+                          const std::optional<torch::Tensor> &k_scale, const std::optional<torch::Tensor> &v_scale,
+                          int64_t window, int64_t sinks, int64_t max_new_len) {
+        return PagedAttentionWorkspace(q, k_pages, v_pages, {kv_indptr, kv_indices, kv_last_page_len, qo_indptr, {}},
+                                       attention_options(k_scale, v_scale, window, sinks, std::nullopt, max_new_len));
+      },
+      py::arg("q"), py::arg("k_pages"), py::arg("v_pages"), py::arg("kv_indptr"), py::arg("kv_indices"),
+      py::arg("kv_last_page_len"), py::arg("qo_indptr"), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(),
+      py::arg("window") = 0, py::arg("sinks") = 0, py::arg("max_new_len") = 0, "workspace bytes of a PagedAttention call");
+
   m.def("SetDistributedInfo", &SetDistributedInfo, py::arg("rank"), py::arg("size"));
   m.def("GetDistributedInfo", []() {
     const auto &d = GetDistributedInfo();

@@ -203,6 +203,55 @@ BatchIndex BuildBatchIndex(const torch::Tensor &prior_len, const torch::Tensor &
                            torch::Dtype slot_dtype = torch::kInt64,
                            const std::optional<torch::Tensor> &error_word = std::nullopt);
 
+// ----------------------------------------------------------------------------
+// 8-bit pool and paged attention (see yl_kv_quant_store, yl_kv_quant_load and
+// yl_paged_attention).  No counterpart in the reference.
+// ----------------------------------------------------------------------------
+
+// K and V as e4m3 codes and one fp32 scale for each page and KV head.
+struct QuantKVPool {
+  torch::Tensor k;        // float8_e4m3fn [P, page_size, H, D] or [L, P, page_size, H, D], any strides, rows contiguous
+  torch::Tensor v;
+  torch::Tensor k_scale;  // fp32 [P, H] or [L, P, H]
+  torch::Tensor v_scale;
+  QuantKVPool Layer(int64_t i) const { return {k.select(0, i), v.select(0, i), k_scale.select(0, i), v_scale.select(0, i)}; }
+};
+
+// A zeroed pool whose pages are stored head-major, so that the tokens that share
+// a scale are contiguous; num_layers 0: no layer dimension.
+QuantKVPool MakeQuantKVPool(int64_t num_pages, int64_t page_size, int64_t num_kv_heads, int64_t head_dim,
+                            int64_t num_layers, torch::Device device);
+
+// k, v: bf16 or fp16 [N, H*D] or [N, H, D], with the pool's layers in front if it
+// has them, in the order of the index.
+void StoreKVCacheQuant(const torch::Tensor &k, const torch::Tensor &v, const QuantKVPool &pool, const BatchIndex &index,
+                       const std::optional<torch::Tensor> &error_word = std::nullopt);
+
+// {k, v} [.., N, H, D] of the slots (int32 or int64 [N]), in `dtype` or into `out`.
+std::pair<torch::Tensor, torch::Tensor> LoadKVCacheQuant(
+    const QuantKVPool &pool, const torch::Tensor &slots, torch::Dtype dtype = torch::kBFloat16,
+    const std::optional<std::pair<torch::Tensor, torch::Tensor>> &out = std::nullopt,
+    const std::optional<torch::Tensor> &error_word = std::nullopt);
+
+struct PagedAttentionOptions {
+  std::optional<torch::Tensor> k_scale;    // of an 8-bit pool
+  std::optional<torch::Tensor> v_scale;
+  int64_t window{0};                       // 0: none
+  int64_t sinks{0};                        // first positions that stay visible beside a window
+  std::optional<double> sm_scale;          // 1 / sqrt(D)
+  int64_t max_new_len{0};                  // most new tokens of one sequence; 0: not known
+  std::optional<torch::Tensor> out;        // like q; else a new tensor
+  std::optional<torch::Tensor> workspace;  // uint8, PagedAttentionWorkspace() bytes; else allocated by the call
+  std::optional<torch::Tensor> error_word;
+};
+
+// q [N, Hq, D], one layer's k_pages, v_pages [P, page_size, H, D] of q's dtype or
+// float8_e4m3fn; returns the output [N, Hq, D].
+torch::Tensor PagedAttention(const torch::Tensor &q, const torch::Tensor &k_pages, const torch::Tensor &v_pages,
+                             const BatchIndex &index, const PagedAttentionOptions &options = {});
+int64_t PagedAttentionWorkspace(const torch::Tensor &q, const torch::Tensor &k_pages, const torch::Tensor &v_pages,
+                                const BatchIndex &index, const PagedAttentionOptions &options = {});
+
 // Make2DIndices (src/include/batch/batch_manager.h:30-51): for each range
 // {row, col_start, col_end} (the first three entries of each tensor, read on
 // the host as the reference does), the indices row + c for c in

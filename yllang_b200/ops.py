@@ -435,17 +435,6 @@ def qkv_norm_rope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cac
     return q_out
 
 
-def _on(device: torch.device, stream: torch.cuda.Stream | None):
-    """Context of a call's allocations and launches: the tensors' device, and
-    the call's stream where one is given (what the call allocates then belongs
-    to the stream that writes it)."""
-    if stream is not None:
-        return torch.cuda.stream(stream)
-    if torch.cuda.current_device() != device.index:
-        return torch.cuda.device(device)
-    return contextlib.nullcontext()
-
-
 class QuantKVPool(NamedTuple):
     """An 8-bit K/V pool: e4m3 codes and one fp32 scale for each page and KV
     head (value = code * scale).
@@ -477,61 +466,34 @@ def quant_kv_pool(num_pages: int, page_size: int, kv_heads: int, head_dim: int, 
     return QuantKVPool(codes[0], codes[1], scales[0], scales[1])
 
 
-def _pool_args(pool: QuantKVPool, what: str) -> _abi.QuantPool:
-    k, v, ks, vs = pool
-    _check(k.dim() in (4, 5), f"{what}: pool.k must be [P, page_size, H, D] or [L, P, page_size, H, D], "
-                              f"got {tuple(k.shape)}")
-    _check(k.is_cuda, f"{what}: the pool must be CUDA tensors")
-    _check(k.dtype == torch.float8_e4m3fn and v.dtype == k.dtype, f"{what}: pool.k and pool.v must be float8_e4m3fn")
-    _check(v.shape == k.shape and v.stride() == k.stride(), f"{what}: pool.k and pool.v must share shape and strides")
-    _check(k.stride(-1) == 1, f"{what}: head rows must be contiguous")
-    _check(ks.dtype == torch.float32 and vs.dtype == torch.float32, f"{what}: scales must be fp32")
-    want = (*k.shape[:-3], k.shape[-2])
-    _check(ks.shape == want and vs.shape == want and ks.stride() == vs.stride(),
-           f"{what}: scales must be {tuple(want)} with equal strides")
-    for name, t in (("v", v), ("k_scale", ks), ("v_scale", vs)):
-        _check(t.device == k.device, f"{what}: pool.{name} on {t.device}, expected {k.device}")
-    a = _abi.QuantPool()
-    a.k_codes, a.v_codes, a.k_scale, a.v_scale = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
-    st, sst = k.stride(), ks.stride()
-    a.page_stride, a.slot_stride, a.head_stride = st[-4], st[-3], st[-2]
-    a.scale_page_stride, a.scale_head_stride = sst[-2], sst[-1]
-    a.num_layers = 1
-    if k.dim() == 5:
-        a.num_layers, a.layer_stride, a.scale_layer_stride = k.shape[0], st[0], sst[0]
-    a.num_pages, a.page_size, a.num_heads, a.head_dim = k.shape[-4:]
-    return a
+def _front_end():
+    """The C++ front end, where the 8-bit pool's and the attention's calls are
+    checked and launched: they run once per layer of a step, and a Python
+    front end of theirs costs more than the smallest of their kernels."""
+    global _C
+    if _C is None:
+        from . import load_extension
+        _C = load_extension()
+    return _C
 
 
-def _check_index(index: BatchIndex, device: torch.device, what: str) -> int:
-    """Check the page arrays an operator reads; returns the batch size."""
-    indptr, indices, last, qo = index[:4]
-    for name, t in (("kv_indptr", indptr), ("kv_indices", indices), ("kv_last_page_len", last), ("qo_indptr", qo)):
-        _check(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.device == device,
-               f"{what}: index.{name} must be contiguous int32 on {device}")
-    B = indptr.shape[0] - 1
-    _check(B >= 0 and qo.shape[0] == B + 1 and last.shape[0] >= B,
-           f"{what}: index needs kv_indptr and qo_indptr [B + 1] and kv_last_page_len [B]")
-    return B
+_C = None
 
 
-_DTYPE = {torch.bfloat16: _abi.YL_DTYPE_BF16, torch.float16: _abi.YL_DTYPE_F16}
-
-
-def _kv_rows(t: torch.Tensor, pool: QuantKVPool, name: str, what: str) -> tuple[int, int, int]:
-    """(tokens, token stride, layer stride) in elements of K/V rows beside a
-    pool: [N, H*D] or [N, H, D], with the pool's layers in front if it has them."""
-    lead = pool.k.dim() - 4
-    H, D = pool.k.shape[-2:]
-    row = tuple(t.shape[lead + 1:])
-    _check(t.dim() > lead and row in ((H * D,), (H, D)) and t.shape[:lead] == pool.k.shape[:lead],
-           f"{what}: {name} must be {[*pool.k.shape[:lead], 'N', H * D]} or {[*pool.k.shape[:lead], 'N', H, D]}, "
-           f"got {tuple(t.shape)}")
-    _check(t.stride(-1) == 1 and (len(row) == 1 or H == 1 or t.stride(-2) == D),
-           f"{what}: {name} rows must be contiguous")
-    N = t.shape[lead]
-    # a single row's stride is arbitrary in torch: give the kernel a valid one
-    return N, t.stride(lead) if N > 1 else H * D, t.stride(0) if lead else 0
+def _run(call, what: str, device: torch.device, stream: torch.cuda.Stream | None, error_word: torch.Tensor | None, args):
+    """One call of the front end on `stream`, its refusals as this module's PanicError."""
+    C = _front_end()
+    try:
+        if stream is None and not CHECK_DEVICE_ERRORS:
+            return call(*args, error_word)
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+            errs = _Errors(error_word, device, what, stream) if device.type == "cuda" else None
+            result = call(*args, error_word if errs is None else errs.tensor)
+        if errs is not None:
+            errs.check()
+        return result
+    except C.PanicError as e:
+        raise PanicError(str(e)) from None
 
 
 def store_kv_cache_quant(k: torch.Tensor, v: torch.Tensor, pool: QuantKVPool, index: BatchIndex,
@@ -546,29 +508,8 @@ def store_kv_cache_quant(k: torch.Tensor, v: torch.Tensor, pool: QuantKVPool, in
     the page's earlier tokens take it too (see yl_kv_quant_store).  Pages that
     two sequences of one call write are outside the contract.  An infinity is
     stored as the largest code and NaN as NaN, with DEVERR_NONFINITE set."""
-    what = "store_kv_cache_quant"
-    p = _pool_args(pool, what)
-    _check(k.dtype in _DTYPE and v.dtype == k.dtype, f"{what}: k and v must both be bf16 or fp16")
-    _check(k.device == pool.k.device and v.device == k.device, f"{what}: k and v must be on the pool's device")
-    N, k_row, k_layer = _kv_rows(k, pool, "k", what)
-    Nv, v_row, v_layer = _kv_rows(v, pool, "v", what)
-    _check(Nv == N, f"{what}: k has {N} rows and v {Nv}")
-    B = _check_index(index, k.device, what)
-    if N == 0 or B == 0:
-        return
-    a = _abi.QuantStoreArgs()
-    a.pool = p
-    a.k, a.v = k.data_ptr(), v.data_ptr()
-    a.kv_indptr, a.kv_indices = index.kv_indptr.data_ptr(), index.kv_indices.data_ptr()
-    a.kv_last_page_len, a.qo_indptr = index.kv_last_page_len.data_ptr(), index.qo_indptr.data_ptr()
-    a.kv_indices_capacity, a.num_tokens, a.batch_size = index.kv_indices.shape[0], N, B
-    a.k_row_stride, a.v_row_stride, a.k_layer_stride, a.v_layer_stride = 2 * k_row, 2 * v_row, 2 * k_layer, 2 * v_layer
-    a.dtype = _DTYPE[k.dtype]
-    with _on(k.device, stream):
-        errs = _Errors(error_word, k.device, what, stream)
-        a.error_word = errs.ptr
-        _abi.check(_abi.kv_quant_store_raw(a, _stream(stream, k.device)))
-    errs.check()
+    _run(_front_end().StoreKVCacheQuant, "store_kv_cache_quant", k.device, stream, error_word,
+         (k, v, *pool, *index[:4]))
 
 
 def load_kv_cache_quant(pool: QuantKVPool, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
@@ -578,39 +519,10 @@ def load_kv_cache_quant(pool: QuantKVPool, slots: torch.Tensor, dtype: torch.dty
     D] for an all-layer pool) in bf16 or fp16, row i from slots[i] (int32 or
     int64 [N], slot = page * page_size + offset, as in slot_mapping).  Slot -1
     gives a zero row, another slot outside the pool a zero row and
-    DEVERR_SLOT_RANGE; values past fp16's range come back as its largest."""
-    what = "load_kv_cache_quant"
-    p = _pool_args(pool, what)
-    dev = pool.k.device
-    _check(slots.dim() == 1 and slots.dtype in (torch.int32, torch.int64) and slots.device == dev
-           and (slots.shape[0] <= 1 or slots.stride(0) == 1),
-           f"{what}: slots must be contiguous int32 or int64 [N] on {dev}")
-    N, H, D = slots.shape[0], p.num_heads, p.head_dim
-    with _on(dev, stream):
-        if out is None:
-            _check(dtype in _DTYPE, f"{what}: dtype must be bf16 or fp16")
-            shape = (*pool.k.shape[:-4], N, H, D)
-            out = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
-        k, v = out
-        _check(k.dtype in _DTYPE and v.dtype == k.dtype and k.device == dev and v.device == dev,
-               f"{what}: out must be two bf16 or two fp16 tensors on {dev}")
-        Nk, k_row, k_layer = _kv_rows(k, pool, "out[0]", what)
-        Nv, v_row, v_layer = _kv_rows(v, pool, "out[1]", what)
-        _check(Nk == N and Nv == N, f"{what}: out must have {N} rows")
-        if N == 0:
-            return out
-        a = _abi.QuantLoadArgs()
-        a.pool = p
-        a.k_out, a.v_out, a.slots, a.num_tokens = k.data_ptr(), v.data_ptr(), slots.data_ptr(), N
-        a.k_row_stride, a.v_row_stride = 2 * k_row, 2 * v_row
-        a.k_layer_stride, a.v_layer_stride = 2 * k_layer, 2 * v_layer
-        a.slot_is_int64 = int(slots.dtype == torch.int64)
-        a.dtype = _DTYPE[k.dtype]
-        errs = _Errors(error_word, dev, what, stream)
-        a.error_word = errs.ptr
-        _abi.check(_abi.kv_quant_load_raw(a, _stream(stream, dev)))
-    errs.check()
-    return out
+    DEVERR_SLOT_RANGE; values past the type's range come back as its largest."""
+    got = _run(_front_end().LoadKVCacheQuant, "load_kv_cache_quant", slots.device, stream, error_word,
+               (*pool, slots, dtype, out))
+    return got if out is None else out
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, index: BatchIndex, *,
@@ -633,93 +545,23 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     tokens of one sequence where the caller knows it (1 for a decode batch),
     which saves launches; sequences of more are skipped with
     DEVERR_TOKEN_COUNT.  Rows behind the last sequence are left as they were
-    (uninitialised in a new `out`).  workspace: uint8 tensor of at least
+    (uninitialised in a new output).  workspace: uint8 tensor of at least
     paged_attention_workspace(...) bytes; by default the call allocates it.
     Calls that may overlap on the GPU need a workspace each."""
-    what = "paged_attention"
-    a, dev = _attention_args(q, k_pages, v_pages, index, k_scale, v_scale, window, sinks, sm_scale, max_new_len)
-    with _on(dev, stream):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        _check(out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.stride(2) == 1,
-               f"{what}: out must be like q, with contiguous heads")
-        if a.num_tokens == 0 or a.batch_size == 0:
-            return out
-        a.o, a.o_row_stride, a.o_head_stride = out.data_ptr(), 2 * out.stride(0), 2 * out.stride(1)
-        need = _abi.paged_attention_workspace_raw(a)
-        if need < 0:
-            _abi.check(int(need))
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        if workspace is not None:
-            _check(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == dev
-                   and workspace.numel() >= need, f"{what}: workspace must be {need} contiguous bytes on {dev}")
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-        errs = _Errors(error_word, dev, what, stream)
-        a.error_word = errs.ptr
-        _abi.check(_abi.paged_attention_raw(a, _stream(stream, dev)))
-    errs.check()
-    return out
+    got = _run(_front_end().PagedAttention, "paged_attention", q.device, stream, error_word,
+               (q, k_pages, v_pages, *index[:4], k_scale, v_scale, window, sinks, sm_scale, max_new_len, out, workspace))
+    return got if out is None else out
 
 
 def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, index: BatchIndex, *,
                               k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
                               window: int = 0, sinks: int = 0, max_new_len: int = 0) -> int:
     """Workspace bytes of a paged_attention call on these tensors."""
-    a, dev = _attention_args(q, k_pages, v_pages, index, k_scale, v_scale, window, sinks, None, max_new_len)
-    with _on(dev, None):
-        need = _abi.paged_attention_workspace_raw(a)
-    if need < 0:
-        _abi.check(int(need))
-    return int(need)
-
-
-def _attention_args(q, k_pages, v_pages, index, k_scale, v_scale, window, sinks, sm_scale, max_new_len):
-    what = "paged_attention"
-    _check(q.dim() == 3 and q.stride(2) == 1, f"{what}: q must be [N, Hq, head_dim] with contiguous heads")
-    _check(q.is_cuda, f"{what}: q must be a CUDA tensor")
-    _check(q.dtype in _DTYPE, f"{what}: q must be bf16 or fp16")
-    dev = q.device
-    _check(k_pages.dim() == 4 and k_pages.stride(3) == 1, f"{what}: k_pages must be [P, page_size, H, D] with "
-                                                          "contiguous head rows")
-    _check(v_pages.shape == k_pages.shape and v_pages.stride() == k_pages.stride() and v_pages.dtype == k_pages.dtype,
-           f"{what}: k_pages and v_pages must share shape, strides and dtype")
-    _check(k_pages.device == dev and v_pages.device == dev, f"{what}: the pool must be on {dev}")
-    N, Hq, D = q.shape
-    P, ps, H, Dk = k_pages.shape
-    _check(Dk == D, f"{what}: head_dim of the pool {Dk} != {D} of q")
-    _check(H > 0 and Hq % H == 0, f"{what}: {Hq} query heads are no multiple of {H} KV heads")
-    item = k_pages.element_size()
-    a = _abi.PagedAttentionArgs()
-    if k_pages.dtype == torch.float8_e4m3fn:
-        _check(k_scale is not None and v_scale is not None, f"{what}: an 8-bit pool needs k_scale and v_scale")
-        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _check(t.dtype == torch.float32 and t.shape == (P, H) and t.device == dev,
-                   f"{what}: {name} must be fp32 [{P}, {H}] on {dev}")
-        _check(k_scale.stride() == v_scale.stride(), f"{what}: k_scale and v_scale must share strides")
-        a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-        a.scale_page_stride, a.scale_head_stride = k_scale.stride()
-        a.kv_dtype = _abi.YL_KV_E4M3
-    else:
-        _check(k_pages.dtype == q.dtype, f"{what}: the pool must be float8_e4m3fn or of q's dtype")
-        _check(k_scale is None and v_scale is None, f"{what}: scales are for 8-bit pools")
-        a.kv_dtype = _abi.YL_KV_SAME
-    B = _check_index(index, dev, what)
-    limit = (1 << 31) - 1
-    _check(0 <= window <= limit and 0 <= sinks <= limit and 0 <= max_new_len <= limit,
-           f"{what}: window, sinks and max_new_len must be in [0, 2^31)")
-    a.q, a.k_cache, a.v_cache = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
-    a.kv_indptr, a.kv_indices = index.kv_indptr.data_ptr(), index.kv_indices.data_ptr()
-    a.kv_last_page_len, a.qo_indptr = index.kv_last_page_len.data_ptr(), index.qo_indptr.data_ptr()
-    a.q_row_stride, a.q_head_stride = 2 * q.stride(0), 2 * q.stride(1)
-    st = k_pages.stride()
-    a.page_stride, a.slot_stride, a.head_stride = item * st[0], item * st[1], item * st[2]
-    a.kv_indices_capacity, a.num_pages, a.num_tokens = index.kv_indices.shape[0], P, N
-    a.batch_size, a.num_q_heads, a.num_kv_heads, a.head_dim, a.page_size = B, Hq, H, D, ps
-    a.dtype = _DTYPE[q.dtype]
-    a.window, a.sinks, a.max_new_len = window, sinks, max_new_len
-    a.sm_scale = D ** -0.5 if sm_scale is None else sm_scale
-    return a, dev
+    C = _front_end()
+    try:
+        return C.PagedAttentionWorkspace(q, k_pages, v_pages, *index[:4], k_scale, v_scale, window, sinks, max_new_len)
+    except C.PanicError as e:
+        raise PanicError(str(e)) from None
 
 
 class DevicePagePool:
