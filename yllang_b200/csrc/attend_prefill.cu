@@ -14,7 +14,7 @@
 //   largest goes to the scores as one factor.  V's are multiplied in relative to
 //   a reference that changes only when a tile's largest passes 64 times it, when
 //   the accumulators are rescaled.
-// * Warp 12 issues the products: S = Q K^T per 128 rows (both operands in shared
+// * Warp 12 (13 to 15 are there for the sharing out of registers) issues the products: S = Q K^T per 128 rows (both operands in shared
 //   memory), O += P V (P in tensor memory).  The two row tiles alternate, so
 //   that one's products run while the other's softmax does.
 // * Warps 0-3 and 4-7 each own a row tile, one row per thread: they write Q into
@@ -38,7 +38,7 @@
 namespace ylk {
 namespace {
 
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 16 * 32;
 constexpr int kLoadThreads = 128;
 constexpr int kStages = 2;
 constexpr float kMoveBy = 8.f;    // log2 of how far weights may pass 1 before their reference moves
@@ -73,6 +73,7 @@ struct Shared {
   uint64_t drained;
   uint32_t tmem;
   float top[2][2][4];           // [parity][K, V][loading warp]: largest scales
+  uint32_t valid[2][4];         // [parity]: tokens with a good page
   TileInfo tile[kStages];
   int64_t offset[2][128];       // [parity]: byte offset of a token's head row
   uint32_t ratio[2][2][128];    // [parity][K, V]: scale over the reference, two halves
@@ -206,161 +207,210 @@ __device__ __forceinline__ uint32_t swizzled(int r, int c) {
   return (c >> 3) * (ROWS * 128) + r * 128 + (((c ^ r) & 7) << 4);
 }
 
+// The tiles of this CTA's items, one after the other.
+struct Tile {
+  int base, cnt;            // first position and tokens of it
+  int e0, head;             // of the sequence; KV head
+  int first_pos, last_pos;  // of the item's queries
+  bool first;               // of its item
+};
+template <int D>
+class Tiles {
+ public:
+  __device__ __forceinline__ Tiles(const AttnParams &p) : walker_(p), n_(blockIdx.x) { more_ = walker_.seek(n_, it_); }
+  // The next tile; false when there is none (cnt is 0 then).
+  __device__ __forceinline__ bool next(Tile &t) {
+    t.cnt = 0;
+    if (!more_) return false;
+    const bool in_head = j_ < it_.head_tiles;
+    t.base = (in_head ? 0 : it_.span.low) + (in_head ? j_ : j_ - it_.head_tiles) * Shape<D>::kKT;
+    t.cnt = min(Shape<D>::kKT, (in_head ? it_.span.head : it_.span.end) - t.base);
+    t.e0 = it_.seq.e0;
+    t.head = it_.head;
+    t.first_pos = it_.first_pos;
+    t.last_pos = it_.last_pos;
+    t.first = j_ == 0;
+    if (++j_ == it_.tiles) {
+      j_ = 0;
+      n_ += gridDim.x;
+      more_ = walker_.seek(n_, it_);
+    }
+    return true;
+  }
+
+ private:
+  Walker<D> walker_;
+  Item it_;
+  int64_t n_;
+  int j_ = 0;
+  bool more_;
+};
+
+// Each thread looks up one token of a tile: its page id two tiles ahead, the
+// page's scales one tile ahead.
 template <typename T, int D, bool Q8>
 __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint8_t *kv) {
   using S = Shape<D>;
   constexpr int KT = S::kKT;
   constexpr bool BF = std::is_same<T, Bf16>::value && !Q8;
+  constexpr int kNone = -0x7fffffff, kNoEntry = -0x7ffffffe;  // not a token of the tile; no such entry
   const int tid = threadIdx.x - 256, lane = tid & 31, warp = tid >> 5;
-  Walker<D> walker(p);
-  Item it;
-  uint32_t used = 0;  // tiles loaded so far
-  for (int64_t n = blockIdx.x; walker.seek(n, it); n += gridDim.x) {
-    float value = 0.f;  // reference of V's scales
-    for (int j = 0; j < it.tiles; ++j, ++used) {
-      const int stage = used % kStages, par = used & 1;
-      const uint32_t phase = (used / kStages & 1) ^ 1;
-      // look-up: one token per thread
-      const bool in_head = j < it.head_tiles;
-      const int base = (in_head ? 0 : it.span.low) + (in_head ? j : j - it.head_tiles) * KT;
-      const int cnt = min(KT, (in_head ? it.span.head : it.span.end) - base);
-      int64_t off = -1;
-      float ks = 0.f, vs = 0.f;
-      if (tid < KT && tid < cnt) {
-        const int pos = base + tid;
-        const int ord = p.by_page.div(pos);
-        const int64_t e = static_cast<int64_t>(it.seq.e0) + ord;
-        if (e >= 0 && e < p.indices_cap) {
-          const int page = __ldg(p.kv_indices + e);
-          if (page >= 0 && page < p.num_pages) {
-            off = static_cast<int64_t>(page) * p.page_stride + static_cast<int64_t>(pos - ord * p.page_size) * p.slot_stride +
-                  it.head * p.head_stride;
-            if (Q8) {
-              const int64_t sc = static_cast<int64_t>(page) * p.scale_page_stride + it.head * p.scale_head_stride;
-              ks = __ldg(p.scale[0] + sc);
-              vs = __ldg(p.scale[1] + sc);
-            }
-          } else {
-            raise_deverr(p.error_word, YL_DEVERR_PAGE_RANGE);
-          }
-        } else {
-          raise_deverr(p.error_word, YL_DEVERR_INDICES_CAP);
-        }
-      }
-      if (tid < KT) sh->offset[par][tid] = off;
-      const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
-      float ktop = ks, vtop = vs;
-      if (Q8) {
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-          ktop = fmaxf(ktop, __shfl_xor_sync(0xffffffffu, ktop, d));
-          vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
-        }
-        if (lane == 0) {
-          sh->top[par][0][warp] = ktop;
-          sh->top[par][1][warp] = vtop;
-        }
-        load_barrier(true);
-        ktop = fmaxf(fmaxf(sh->top[par][0][0], sh->top[par][0][1]), fmaxf(sh->top[par][0][2], sh->top[par][0][3]));
-        vtop = fmaxf(fmaxf(sh->top[par][1][0], sh->top[par][1][1]), fmaxf(sh->top[par][1][2], sh->top[par][1][3]));
-      }
-      float move = 1.f;
-      if (Q8) {
-        if (vtop > value * kMaxRatio) {
-          move = value / vtop;
-          value = vtop;
-        }
-        if (tid < KT) {
-          const float rk = ktop > 0.f ? ks / ktop : 0.f, rv = value > 0.f ? vs / value : 0.f;
-          sh->ratio[par][0][tid] = Fp16::pack(rk, rk);
-          sh->ratio[par][1][tid] = Fp16::pack(rv, rv);
-        }
-      }
-      // the stage's previous tile is used up, its description too
-      const bool fine = wait_or_report(p, &sh->k_empty[stage], phase) && wait_or_report(p, &sh->v_empty[stage], phase);
-      TileInfo *info = &sh->tile[stage];
-      if (lane == 0 && warp * 32 < KT) {
-        info->valid[warp] = ok;
-        info->ghost[warp] = 0;
-      }
-      if (!load_barrier(fine)) return;
-      // a tile with a bad page is masked like one that some row sees in part
-      uint32_t all = 0xffffffffu;
-#pragma unroll
-      for (int k = 0; k < KT / 32; ++k) all &= info->valid[k];
-      const bool edge = all != 0xffffffffu || base + KT - 1 > it.first_pos ||
-                        (p.window > 0 && base <= it.last_pos - p.window && base + KT > p.sinks);
-      if (tid == 0) {
-        info->key = Q8 && ktop > 0.f ? ktop : 1.f;
-        info->move = move;
-        info->value = Q8 ? value : 1.f;
-        info->base = base;
-        info->edge = edge;
-      }
+  Tiles<D> tiles(p);
+  auto page_of = [&](const Tile &t) {
+    if (tid >= KT || tid >= t.cnt) return kNone;
+    const int64_t e = static_cast<int64_t>(t.e0) + p.by_page.div(t.base + tid);
+    return e >= 0 && e < p.indices_cap ? __ldg(p.kv_indices + e) : kNoEntry;
+  };
+  auto good = [&](int page) { return page >= 0 && page < p.num_pages; };
+  auto scales_of = [&](const Tile &t, int page, float &ks, float &vs) {
+    ks = vs = 0.f;
+    if (Q8 && good(page)) {
+      const int64_t sc = static_cast<int64_t>(page) * p.scale_page_stride + t.head * p.scale_head_stride;
+      ks = __ldg(p.scale[0] + sc);
+      vs = __ldg(p.scale[1] + sc);
+    }
+  };
+  Tile t0, t1, t2;
+  bool more0 = tiles.next(t0), more1 = tiles.next(t1);
+  int page0 = more0 ? page_of(t0) : kNone, page1 = more1 ? page_of(t1) : kNone;
+  float ks0, vs0;
+  scales_of(t0, page0, ks0, vs0);
+  float value = 0.f;  // reference of V's scales
+  for (uint32_t used = 0; more0; ++used) {
+    const int stage = used % kStages, par = used & 1;
+    const uint32_t phase = (used / kStages & 1) ^ 1;
+    const bool more2 = tiles.next(t2);
+    const int page2 = more2 ? page_of(t2) : kNone;
+    float ks1 = 0.f, vs1 = 0.f;
+    if (more1) scales_of(t1, page1, ks1, vs1);
 
-      const uint32_t sk = smem_addr(kv + stage * 2 * S::kKVBytes), sv = sk + S::kKVBytes;
-      if (Q8) {
-        constexpr int CH = D / 16;                     // 16-byte chunks of a token's codes
-        constexpr int PER = KT * CH / kLoadThreads;    // of a thread
-        static_assert(PER % 4 == 0, "");
-        const int c = tid % CH, r0 = tid / CH;
-        uint4 w[2][PER];
+    int64_t off = -1;
+    if (good(page0)) {
+      const int pos = t0.base + tid;
+      off = static_cast<int64_t>(page0) * p.page_stride +
+            static_cast<int64_t>(pos - static_cast<int>(p.by_page.div(pos)) * p.page_size) * p.slot_stride +
+            t0.head * p.head_stride;
+    } else if (page0 != kNone) {
+      raise_deverr(p.error_word, page0 == kNoEntry ? YL_DEVERR_INDICES_CAP : YL_DEVERR_PAGE_RANGE);
+    }
+    if (tid < KT) sh->offset[par][tid] = off;
+    const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
+    if (lane == 0 && warp * 32 < KT) sh->valid[par][warp] = ok;
+    if (Q8) {
+      float ktop = ks0, vtop = vs0;
 #pragma unroll
-        for (int kv_i = 0; kv_i < 2; ++kv_i)
+      for (int d = 16; d > 0; d >>= 1) {
+        ktop = fmaxf(ktop, __shfl_xor_sync(0xffffffffu, ktop, d));
+        vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
+      }
+      if (lane == 0) {
+        sh->top[par][0][warp] = ktop;
+        sh->top[par][1][warp] = vtop;
+      }
+    }
+    load_barrier(true);
+    float key = 1.f, move = 1.f;
+    if (t0.first) value = Q8 ? 0.f : 1.f;
+    if (Q8) {
+      const float ktop = fmaxf(fmaxf(sh->top[par][0][0], sh->top[par][0][1]), fmaxf(sh->top[par][0][2], sh->top[par][0][3]));
+      const float vtop = fmaxf(fmaxf(sh->top[par][1][0], sh->top[par][1][1]), fmaxf(sh->top[par][1][2], sh->top[par][1][3]));
+      if (ktop > 0.f) key = ktop;
+      if (vtop > value * kMaxRatio) {
+        move = value / vtop;
+        value = vtop;
+      }
+      if (tid < KT) {
+        const float rk = ks0 / key, rv = value > 0.f ? vs0 / value : 0.f;
+        sh->ratio[par][0][tid] = Fp16::pack(rk, rk);
+        sh->ratio[par][1][tid] = Fp16::pack(rv, rv);
+      }
+    }
+    // a tile with a bad page is masked like one that some row sees in part
+    uint32_t all = 0xffffffffu;
 #pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const int64_t o = sh->offset[par][r0 + i * (kLoadThreads / CH)];
-            w[kv_i][i] = make_uint4(0, 0, 0, 0);
-            if (o >= 0) w[kv_i][i] = __ldg(reinterpret_cast<const uint4 *>(p.kv[kv_i] + o + c * 16));
-          }
+    for (int k = 0; k < KT / 32; ++k) all &= sh->valid[par][k];
+    const bool edge = all != 0xffffffffu || t0.base + KT - 1 > t0.first_pos ||
+                      (p.window > 0 && t0.base <= t0.last_pos - p.window && t0.base + KT > p.sinks);
+    const uint32_t sk = smem_addr(kv + stage * 2 * S::kKVBytes), sv = sk + S::kKVBytes;
+    constexpr int CH = D * (Q8 ? 1 : 2) / 16;    // 16-byte chunks of a token's head row
+    constexpr int STEP = kLoadThreads / CH;      // rows of one pass of the threads
+    constexpr int PER = KT / STEP;               // chunks of a thread
+    const int c = tid % CH, r0 = tid / CH;
+    uint4 w[Q8 ? PER : 1];
+    if (Q8) {  // K's codes are on their way before the stage is free
 #pragma unroll
-        for (int kv_i = 0; kv_i < 2; ++kv_i) {
+      for (int i = 0; i < PER; ++i) {
+        const int64_t o = sh->offset[par][r0 + i * STEP];
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (o >= 0) w[i] = __ldg(reinterpret_cast<const uint4 *>(p.kv[0] + o + c * 16));
+      }
+    }
+    // the stage's previous tile is used up, its description too
+    const bool fine = wait_or_report(p, &sh->k_empty[stage], phase) && wait_or_report(p, &sh->v_empty[stage], phase);
+    TileInfo *info = &sh->tile[stage];
+    if (tid == 0) {
+      info->key = key;
+      info->move = move;
+      info->value = value;
+      info->base = t0.base;
+      info->edge = edge;
+    }
+    if (tid < KT / 32) {
+      info->valid[tid] = sh->valid[par][tid];
+      info->ghost[tid] = 0;
+    }
+    if (!load_barrier(fine)) break;
+
+    if (Q8) {
+      auto convert = [&](int i, int r, int kv_i) {
+        const uint32_t ratio = sh->ratio[par][kv_i][r];
+        const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        uint32_t y[8];
 #pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const int r = r0 + i * (kLoadThreads / CH);
-            const uint32_t ratio = sh->ratio[par][kv_i][r];
-            const uint32_t x[4] = {w[kv_i][i].x, w[kv_i][i].y, w[kv_i][i].z, w[kv_i][i].w};
-            uint32_t y[8];
-            uint32_t any = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              y[2 * k] = mul_half2(e4m3x2_to_half2(static_cast<uint16_t>(x[k])), ratio);
-              y[2 * k + 1] = mul_half2(e4m3x2_to_half2(static_cast<uint16_t>(x[k] >> 16)), ratio);
-            }
-            if (kv_i == 1 && edge) {
-#pragma unroll
-              for (int k = 0; k < 8; ++k) any |= drop_nonfinite<false>(y[k]);
-              if (any) atomicOr(&info->ghost[r >> 5], 1u << (r & 31));
-            }
-            const uint32_t at = kv_i ? sv : sk;
-            sts128(at + swizzled<KT>(r, 2 * c), y[0], y[1], y[2], y[3]);
-            sts128(at + swizzled<KT>(r, 2 * c + 1), y[4], y[5], y[6], y[7]);
-          }
-          fence_to_async();
-          mbar_arrive(kv_i ? &sh->v_full[stage] : &sh->k_full[stage]);
+        for (int k = 0; k < 4; ++k) {
+          y[2 * k] = mul_half2(e4m3x2_to_half2(static_cast<uint16_t>(x[k])), ratio);
+          y[2 * k + 1] = mul_half2(e4m3x2_to_half2(static_cast<uint16_t>(x[k] >> 16)), ratio);
         }
-      } else {
-        constexpr int CH = D / 8;
-        constexpr int PER = KT * CH / kLoadThreads;
-        const int c = tid % CH, r0 = tid / CH;
+        if (kv_i == 1 && edge) {
+          uint32_t any = 0;
 #pragma unroll
-        for (int kv_i = 0; kv_i < 2; ++kv_i) {
-#pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const int r = r0 + i * (kLoadThreads / CH);
-            const int64_t o = sh->offset[par][r];
-            cp_async16((kv_i ? sv : sk) + swizzled<KT>(r, c), p.kv[kv_i] + (o >= 0 ? o + c * 16 : 0), o >= 0);
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
+          for (int k = 0; k < 8; ++k) any |= drop_nonfinite<false>(y[k]);
+          if (any) atomicOr(&info->ghost[r >> 5], 1u << (r & 31));
         }
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        fence_to_async();
-        mbar_arrive(&sh->k_full[stage]);
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        if (edge) {
+        const uint32_t at = kv_i ? sv : sk;
+        sts128(at + swizzled<KT>(r, 2 * c), y[0], y[1], y[2], y[3]);
+        sts128(at + swizzled<KT>(r, 2 * c + 1), y[4], y[5], y[6], y[7]);
+      };
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int r = r0 + i * STEP;
+        convert(i, r, 0);
+        const int64_t o = sh->offset[par][r];
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (o >= 0) w[i] = __ldg(reinterpret_cast<const uint4 *>(p.kv[1] + o + c * 16));
+      }
+      fence_to_async();
+      mbar_arrive(&sh->k_full[stage]);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) convert(i, r0 + i * STEP, 1);
+      fence_to_async();
+      mbar_arrive(&sh->v_full[stage]);
+    } else {
+#pragma unroll
+      for (int kv_i = 0; kv_i < 2; ++kv_i) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int r = r0 + i * STEP;
+          const int64_t o = sh->offset[par][r];
+          cp_async16((kv_i ? sv : sk) + swizzled<KT>(r, c), p.kv[kv_i] + (o >= 0 ? o + c * 16 : 0), o >= 0);
+        }
+        if (kv_i == 0 || !edge) {
+          cp_async_arrive(smem_addr(kv_i ? &sh->v_full[stage] : &sh->k_full[stage]));  // when they have landed
+        } else {
+          cp_async_wait_all();
 #pragma unroll 1
           for (int i = 0; i < PER; ++i) {  // the chunks that this thread copied
-            const int r = r0 + i * (kLoadThreads / CH);
+            const int r = r0 + i * STEP;
             const uint32_t at = sv + swizzled<KT>(r, c);
             uint32_t x[4];
             asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at));
@@ -372,12 +422,20 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
               sts128(at, x[0], x[1], x[2], x[3]);
             }
           }
+          mbar_arrive(&sh->v_full[stage]);
         }
-        fence_to_async();
-        mbar_arrive(&sh->v_full[stage]);
       }
     }
+    t0 = t1;
+    t1 = t2;
+    more0 = more1;
+    more1 = more2;
+    page0 = page1;
+    page1 = page2;
+    ks0 = ks1;
+    vs0 = vs1;
   }
+  cp_async_wait_all();
 }
 
 // ---------------------------------------------------------------------------
@@ -409,6 +467,7 @@ __device__ __forceinline__ void issue_products(const AttnParams &p, Shared *sh, 
         if (w == live - 1) mma_commit(&sh->k_empty[tile % kStages]);
       };
       ok = wait_or_report(p, &sh->k_full[used % kStages], used / kStages & 1);
+      fence_to_async();  // (asynchronous copies of a 16-bit pool arrive without one)
       for (int w = 0; w < live && ok; ++w) {
         ok = wait_or_report(p, &sh->q_full[w], queries[w]++ & 1);
         if (!ok) break;
@@ -418,6 +477,7 @@ __device__ __forceinline__ void issue_products(const AttnParams &p, Shared *sh, 
       for (int j = 0; j < it.tiles && ok; ++j) {
         const uint32_t tile = used + j;
         ok = wait_or_report(p, &sh->v_full[tile % kStages], tile / kStages & 1);
+        fence_to_async();
         for (int w = 0; w < live && ok; ++w) {
           ok = wait_or_report(p, &sh->p_full[w], weights[w]++ & 1);
           if (!ok) break;
@@ -429,9 +489,11 @@ __device__ __forceinline__ void issue_products(const AttnParams &p, Shared *sh, 
                    j > 0 || s > 0);
           if (w == live - 1) mma_commit(&sh->v_empty[tile % kStages]);
           if (j + 1 < it.tiles) {
-            if (w == 0) ok = wait_or_report(p, &sh->k_full[(tile + 1) % kStages], (tile + 1) / kStages & 1);
-            if (!ok) break;
-            tc_fence_after();
+            if (w == 0) {
+              ok = wait_or_report(p, &sh->k_full[(tile + 1) % kStages], (tile + 1) / kStages & 1);
+              if (!ok) break;
+              fence_to_async();
+            }
             scores(w, tile + 1);
           } else {
             mma_commit(&sh->o_full[w]);
@@ -453,6 +515,24 @@ __device__ __forceinline__ void issue_products(const AttnParams &p, Shared *sh, 
 // ---------------------------------------------------------------------------
 // Softmax warps: row tile w, one row per thread
 // ---------------------------------------------------------------------------
+// The lowest n bits, n of any sign.
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+
+// This row's accumulator times a factor (rare: the reference of the weights moved).
+template <int D>
+__device__ __forceinline__ void rescale(uint32_t at, float factor) {
+#pragma unroll 1
+  for (int k = 0; k < D / 32; ++k) {
+    uint32_t x[32];
+    tmem_ld32(at + 32 * k, x);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * factor);
+    tmem_st32(at + 32 * k, x);
+  }
+}
+
 template <typename T, int D, bool Q8>
 __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, uint8_t *q, int w) {
   using S = Shape<D>;
@@ -530,27 +610,44 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
       const bool edge = info->edge != 0;
       value = info->value;
       if (edge && !warp_wait(p, &sh->v_full[stage], phase)) return;  // which values were no numbers
-      auto mask = [&](uint32_t (&x)[32], int k) {
-        const uint32_t valid = info->valid[k], ghost = info->ghost[k];
-        const int first = info->base + 32 * k;
+      // The scores in chunks of 64 columns: the maximum over all, the last chunk
+      // first; then the weights, the first chunk first (it is still in registers),
+      // each written over scores that are used up.
+      uint32_t x[64];
+      auto load = [&](int h) {
+        tmem_ld64(ts + 64 * h, x);
+        if (edge) {
+          // columns that this row sees: up to `last`, and past `out` or before `sink`
+          const int base = info->base + 64 * h;
+          const int last = pos - base + 1, out = p.window > 0 ? pos - p.window - base + 1 : 0;
+          const int sink = p.window > 0 ? p.sinks - base : 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (!((valid >> i) & 1u) || !sees(p, pos, first + i))
-            x[i] = 0xff800000u;  // -inf
-          else if ((ghost >> i) & 1u)
-            x[i] = 0x7fffffffu;  // NaN
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t see =
+                info->valid[2 * h + k] & low_bits(last - 32 * k) & (~low_bits(out - 32 * k) | low_bits(sink - 32 * k));
+            const uint32_t ghost = info->ghost[2 * h + k] & see;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((see >> i) & 1u)) x[32 * k + i] = 0xff800000u;  // -inf
+            if (ghost) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if ((ghost >> i) & 1u) x[32 * k + i] = 0x7fffffffu;  // NaN
+            }
+          }
         }
       };
-      float top = -INFINITY;
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int k = 0; k < KT / 32; ++k) {
-        uint32_t x[32];
-        tmem_ld32(ts + 32 * k, x);
-        if (edge) mask(x, k);
+      for (int h = KT / 64 - 1; h >= 0; --h) {
+        load(h);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
+        for (int i = 0; i < 64; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tops[k] = fmaxf(tops[k], fmaxf(__uint_as_float(x[i + 2 * k]), __uint_as_float(x[i + 2 * k + 1])));
       }
-      top *= c;
+      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * c;
       float factor = move;
       if (top > m + kMoveBy) {
         const float f = fast_exp2(m - top);
@@ -558,34 +655,25 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
         l *= f;
         factor *= f;
       }
-      if (j > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          uint32_t x[32];
-          tmem_ld32(to + 32 * k, x);
-  #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * factor);
-          tmem_st32(to + 32 * k, x);
-        }
-      }
+      const bool moved = j > 0 && __any_sync(0xffffffffu, factor != 1.f);
       const float off = kLift - (m == -INFINITY ? 0.f : m);
-      float sum0 = 0.f, sum1 = 0.f;
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < KT / 32; ++k) {
-        uint32_t x[32], y[16];
-        tmem_ld32(ts + 32 * k, x);
-        if (edge) mask(x, k);
+      for (int h = 0; h < KT / 64; ++h) {
+        if (h > 0) load(h);
+        uint32_t y[32];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < 32; ++i) {
           const float a = fast_exp2(fmaf(__uint_as_float(x[2 * i]), c, off));
           const float b = fast_exp2(fmaf(__uint_as_float(x[2 * i + 1]), c, off));
-          sum0 += a;
-          sum1 += b;
+          sums[2 * (i & 1)] += a;
+          sums[2 * (i & 1) + 1] += b;
           y[i] = BF ? Bf16::pack(a, b) : Fp16::pack(a, b);
         }
-        tmem_st16(ts + 16 * k, y);  // over scores that are read
+        tmem_st32(ts + 32 * h, y);
       }
-      l += sum0 + sum1;
+      if (moved) rescale<D>(to, factor);
+      l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&sh->p_full[w]);
@@ -642,12 +730,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp < 8)
+  // registers of the launch (512 x 128) shared out by role: 256 x 152 + 128 x 112 + 128 x 96
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     softmax_rows<T, D, Q8>(p, sh, q, warp >> 2);
-  else if (warp < 12)
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     load_tiles<T, D, Q8>(p, sh, kv);
-  else
-    issue_products<T, D, Q8>(p, sh, q, kv);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == 12) issue_products<T, D, Q8>(p, sh, q, kv);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
