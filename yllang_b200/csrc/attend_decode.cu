@@ -350,7 +350,7 @@ __device__ __forceinline__ void load_units(const AttnParams &p, const Place &pla
       }
       look_up();
     }
-    if (!mbar_wait_bounded(empty + stage, phase, kBulkWaitLimitNs)) {
+    if (!mbar_wait_clocked(empty + stage, phase)) {
       if (lane == 0) raise_deverr(p.error_word, YL_DEVERR_TIMEOUT);
       break;
     }
@@ -458,7 +458,7 @@ __device__ __forceinline__ void compute_units(const AttnParams &p, const Place &
   for (int u = 0; u < count; ++u) {
     uint8_t *st = stages + stage * L::kStage;
     const uint32_t sk = smem_addr(st), sv = sk + L::kKV, sq = sv + L::kKV, ss = sq + L::kQ;
-    if (!mbar_wait_bounded(full + stage, phase, kBulkWaitLimitNs)) {
+    if (!mbar_wait_clocked(full + stage, phase)) {
       if (lane == 0) raise_deverr(p.error_word, YL_DEVERR_TIMEOUT);
       return;
     }
@@ -720,7 +720,7 @@ __device__ __forceinline__ void compute_units(const AttnParams &p, const Place &
     auto meet = [&]() -> bool {
       __syncwarp();
       if (lane == 0) mbar_arrive(joined);
-      const bool ok = mbar_wait_bounded(joined, join_phase, kBulkWaitLimitNs);
+      const bool ok = mbar_wait_clocked(joined, join_phase);
       join_phase ^= 1;
       if (!ok && lane == 0) raise_deverr(p.error_word, YL_DEVERR_TIMEOUT);
       return ok;
@@ -839,6 +839,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, Q8, NB>::kCtas)
     mbar_init(joined, kConsumers);
   }
   pdl_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.items = 0;
   Place place;
   const bool work = find_place<L>(p, place);  // synchronises the block
   pdl_trigger();
@@ -931,7 +932,7 @@ int64_t decode_workspace(const yl_paged_attention_args *a, int64_t most_rows) {
   return pick(a->dtype, a->head_dim, a->kv_dtype == YL_KV_E4M3, most_rows, [](auto, auto d, auto q, auto b) {
     using L = Layout<decltype(d)::value, decltype(q)::value, decltype(b)::value>;
     const int64_t ctas = static_cast<int64_t>(sm_count()) * L::kCtas;
-    return ctas * 16 + ctas * 2 * (L::kRows * decltype(d)::value + 2 * L::kRows) * 4;
+    return 16 + ctas * 16 + ctas * 2 * (L::kRows * decltype(d)::value + 2 * L::kRows) * 4;
   });
 }
 
@@ -942,8 +943,9 @@ int launch_decode(AttnParams &p, const yl_paged_attention_args *a, int64_t most_
     constexpr bool Q8 = decltype(q)::value;
     using L = Layout<D, Q8, NB>;
     const int ctas = sm_count() * L::kCtas;
-    p.meta = static_cast<int4 *>(a->workspace);
-    p.partials = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + static_cast<int64_t>(ctas) * 16);
+    p.items = static_cast<int *>(a->workspace);
+    p.meta = reinterpret_cast<int4 *>(static_cast<char *>(a->workspace) + 16);
+    p.partials = reinterpret_cast<float *>(p.meta + ctas);
     int rc = allow_smem(reinterpret_cast<const void *>(decode_kernel<T, D, Q8, NB>), L::kSmem);
     if (rc != YL_OK) return rc;
     rc = launch_dependent(decode_kernel<T, D, Q8, NB>, dim3(ctas), dim3(kThreads), L::kSmem, stream,

@@ -25,6 +25,7 @@ struct AttnParams {
   uint32_t *error_word;
   float *partials;  // decode: unfinished results of the CTAs
   int4 *meta;       // decode: where CTA c's first segment has its parts
+  int *items;       // prefill: items taken beyond each CTA's first; the decode kernel before it zeroes it
   int32_t num_pages, batch, heads, group, page_size, window, sinks, max_new;
   int32_t max_rows;  // sequences of at most this many (token, head of a group) rows are the decode kernel's
   FastDiv by_page, by_group;

@@ -4,9 +4,10 @@
 //
 // A work item is 2 x 128 query rows of one (sequence, KV head), a row being a
 // (new token, head of the group), so a tile of keys serves the whole group.
-// One CTA per SM walks items; its warps have fixed roles:
+// One CTA per SM takes items from a counter, the rows that see most first; its
+// warps have fixed roles:
 //
-// * Warps 8-11 load: they gather rows of K and V by page, in tiles of KT tokens,
+// * Warps 16-23 load: they gather rows of K and V by page, in tiles of KT tokens,
 //   and leave them 16-bit and swizzled in a ring of two stages.  16-bit pools
 //   are copied asynchronously; the codes of an 8-bit pool are converted on the
 //   way to fp16, which holds every e4m3 value.  K's scales, relative to the
@@ -14,15 +15,19 @@
 //   largest goes to the scores as one factor.  V's are multiplied in relative to
 //   a reference that changes only when a tile's largest passes 64 times it, when
 //   the accumulators are rescaled.
-// * Warp 12 (13 to 15 are there for the sharing out of registers) issues the products: S = Q K^T per 128 rows (both operands in shared
+// * Warp 24 issues the products: S = Q K^T per 128 rows (both operands in shared
 //   memory), O += P V (P in tensor memory).  The two row tiles alternate, so
-//   that one's products run while the other's softmax does.
-// * Warps 0-3 and 4-7 each own a row tile, one row per thread: they write Q into
-//   shared memory (bf16 queries of an 8-bit pool become fp16 by a power of two
-//   per row), then per tile of keys read S, keep the running maximum and sum in
-//   fp32, and write the weights over S in 16 bits.  The maximum that the weights
-//   refer to moves only when it grew by more than 2^8; then the row's
-//   accumulator is rescaled.  fp16 weights are kept times 2^7, at most 2^15.
+//   that one's products run while the other's softmax does.  Warp 25 plans: it
+//   finds the items and describes their tiles to the others, some ahead.  (Warps
+//   26 and 27 are there for the sharing out of registers.)
+// * Warps 0-7 and 8-15 each own a row tile, two threads per row, a half of the
+//   columns each: one warp per scheduler would leave the exponentials waiting
+//   for one another's latency.  They write Q into shared memory (bf16 queries of
+//   an 8-bit pool become fp16 by a power of two per row), then per tile of keys
+//   read S once and write the weights over it in 16 bits.  The weights refer to
+//   an earlier tile's maximum: that is looked at again, and the row's accumulator
+//   rescaled, only where a sum of weights shows that one may have grown past
+//   2^8 (fp16 weights are kept times 2^7).
 //
 // Only tiles that some row does not see in full are masked; in those, infinities
 // and NaN of V are zeroed as they are loaded and reported to the rows that see
@@ -38,10 +43,13 @@
 namespace ylk {
 namespace {
 
-constexpr int kThreads = 16 * 32;
-constexpr int kLoadThreads = 128;
+constexpr int kSoftmaxWarps = 16, kLoadWarps = 8;
+constexpr int kThreads = (kSoftmaxWarps + kLoadWarps + 4) * 32;
+constexpr int kLoadThreads = kLoadWarps * 32;
+constexpr int kTileThreads = 256;  // softmax threads of a row tile
 constexpr int kStages = 2;
 constexpr float kMoveBy = 8.f;    // log2 of how far weights may pass 1 before their reference moves
+constexpr float kMost = 32768.f;  // sum of weights of half a row, lift included, above which they are looked at again
 constexpr float kMaxRatio = 64.f; // of a V scale to the reference
 
 template <int D>
@@ -63,20 +71,43 @@ struct TileInfo {
   float value;       // what the accumulators are multiples of, from this tile on
   int base;          // position of the first token
   int edge;          // some row does not see every token
+  int live;          // row tiles of the item; 0: there are no more tiles
+  int last;          // of its item
   uint32_t valid[4]; // tokens with a good page
   uint32_t ghost[4]; // edge tiles: tokens whose V had an infinity or NaN
 };
 
+// The planning warp's word on a tile.
+struct Plan {
+  int base, cnt;            // first position and tokens of it
+  int e0, head;             // of the sequence; KV head
+  int first_pos, last_pos;  // of the item's queries
+  int live;                 // row tiles of the item; 0: there are no more tiles
+  int flags;                // kFirst | kLast of its item
+};
+constexpr int kFirst = 1, kLast = 2, kPlans = 4;
+
+// And on an item.
+struct ItemInfo {
+  int tiles;  // 0: there are no more items
+  int q0, fresh, total;
+  int head, row0, rows;
+};
+
 struct Shared {
   uint64_t k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages];
+  uint64_t item_full[2], item_empty[2], plan_full[kPlans], plan_empty[kPlans];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
   uint64_t drained;
   uint32_t tmem;
-  float top[2][2][4];           // [parity][K, V][loading warp]: largest scales
-  uint32_t valid[2][4];         // [parity]: tokens with a good page
+  float top[2][2][kLoadWarps];     // [parity][K, V][loading warp]: largest scales
+  uint32_t valid[2][4];            // [parity]: tokens with a good page
   TileInfo tile[kStages];
-  int64_t offset[2][128];       // [parity]: byte offset of a token's head row
-  uint32_t ratio[2][2][128];    // [parity][K, V]: scale over the reference, two halves
+  ItemInfo item[2];
+  Plan plan[kPlans];
+  int64_t offset[2][128];          // [parity]: byte offset of a token's head row
+  uint32_t ratio[2][2][128];       // [parity][K, V]: scale over the reference, two halves
+  float rows[2][2][128];           // [row tile][half of the columns]: a row's maximum or sum
 };
 static_assert(sizeof(Shared) <= 8192, "shared header");
 
@@ -155,13 +186,13 @@ class Walker {
 };
 
 __device__ __forceinline__ bool wait_or_report(const AttnParams &p, uint64_t *bar, uint32_t parity) {
-  if (mbar_wait_bounded(bar, parity, kBulkWaitLimitNs)) return true;
+  if (mbar_wait_clocked(bar, parity)) return true;
   raise_deverr(p.error_word, YL_DEVERR_TIMEOUT);
   return false;
 }
-// The same answer for the whole warp, which then goes on or leaves together.
+// The same answer for the whole warp.
 __device__ __forceinline__ bool warp_wait(const AttnParams &p, uint64_t *bar, uint32_t parity) {
-  const bool ok = mbar_wait_bounded(bar, parity, kBulkWaitLimitNs);
+  const bool ok = mbar_wait_clocked(bar, parity);
   if (!ok) raise_deverr(p.error_word, YL_DEVERR_TIMEOUT);
   return __all_sync(0xffffffffu, ok);
 }
@@ -172,13 +203,29 @@ __device__ __forceinline__ bool load_barrier(bool fine) {
       "{\n"
       ".reg .pred p, q;\n"
       "setp.ne.u32 q, %1, 0;\n"
-      "barrier.cta.red.and.pred p, 1, 128, q;\n"
+      "barrier.cta.red.and.pred p, 1, 256, q;\n"
       "selp.u32 %0, 1, 0, p;\n"
       "}\n"
       : "=r"(all)
       : "r"(static_cast<uint32_t>(fine))
       : "memory");
   return all != 0;
+}
+
+// Barrier of a row tile's softmax threads; whether any of them passed true.
+__device__ __forceinline__ bool tile_barrier(int w, bool any) {
+  uint32_t r;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.u32 q, %1, 0;\n"
+      "barrier.cta.red.or.pred p, %2, 256, q;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(any)), "r"(2 + w)
+      : "memory");
+  return r != 0;
 }
 
 // ---------------------------------------------------------------------------
@@ -207,45 +254,6 @@ __device__ __forceinline__ uint32_t swizzled(int r, int c) {
   return (c >> 3) * (ROWS * 128) + r * 128 + (((c ^ r) & 7) << 4);
 }
 
-// The tiles of this CTA's items, one after the other.
-struct Tile {
-  int base, cnt;            // first position and tokens of it
-  int e0, head;             // of the sequence; KV head
-  int first_pos, last_pos;  // of the item's queries
-  bool first;               // of its item
-};
-template <int D>
-class Tiles {
- public:
-  __device__ __forceinline__ Tiles(const AttnParams &p) : walker_(p), n_(blockIdx.x) { more_ = walker_.seek(n_, it_); }
-  // The next tile; false when there is none (cnt is 0 then).
-  __device__ __forceinline__ bool next(Tile &t) {
-    t.cnt = 0;
-    if (!more_) return false;
-    const bool in_head = j_ < it_.head_tiles;
-    t.base = (in_head ? 0 : it_.span.low) + (in_head ? j_ : j_ - it_.head_tiles) * Shape<D>::kKT;
-    t.cnt = min(Shape<D>::kKT, (in_head ? it_.span.head : it_.span.end) - t.base);
-    t.e0 = it_.seq.e0;
-    t.head = it_.head;
-    t.first_pos = it_.first_pos;
-    t.last_pos = it_.last_pos;
-    t.first = j_ == 0;
-    if (++j_ == it_.tiles) {
-      j_ = 0;
-      n_ += gridDim.x;
-      more_ = walker_.seek(n_, it_);
-    }
-    return true;
-  }
-
- private:
-  Walker<D> walker_;
-  Item it_;
-  int64_t n_;
-  int j_ = 0;
-  bool more_;
-};
-
 // Each thread looks up one token of a tile: its page id two tiles ahead, the
 // page's scales one tile ahead.
 template <typename T, int D, bool Q8>
@@ -254,15 +262,14 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
   constexpr int KT = S::kKT;
   constexpr bool BF = std::is_same<T, Bf16>::value && !Q8;
   constexpr int kNone = -0x7fffffff, kNoEntry = -0x7ffffffe;  // not a token of the tile; no such entry
-  const int tid = threadIdx.x - 256, lane = tid & 31, warp = tid >> 5;
-  Tiles<D> tiles(p);
-  auto page_of = [&](const Tile &t) {
+  const int tid = threadIdx.x - kSoftmaxWarps * 32, lane = tid & 31, warp = tid >> 5;
+  auto page_of = [&](const Plan &t) {
     if (tid >= KT || tid >= t.cnt) return kNone;
     const int64_t e = static_cast<int64_t>(t.e0) + p.by_page.div(t.base + tid);
     return e >= 0 && e < p.indices_cap ? __ldg(p.kv_indices + e) : kNoEntry;
   };
   auto good = [&](int page) { return page >= 0 && page < p.num_pages; };
-  auto scales_of = [&](const Tile &t, int page, float &ks, float &vs) {
+  auto scales_of = [&](const Plan &t, int page, float &ks, float &vs) {
     ks = vs = 0.f;
     if (Q8 && good(page)) {
       const int64_t sc = static_cast<int64_t>(page) * p.scale_page_stride + t.head * p.scale_head_stride;
@@ -270,19 +277,27 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
       vs = __ldg(p.scale[1] + sc);
     }
   };
-  Tile t0, t1, t2;
-  bool more0 = tiles.next(t0), more1 = tiles.next(t1);
-  int page0 = more0 ? page_of(t0) : kNone, page1 = more1 ? page_of(t1) : kNone;
-  float ks0, vs0;
-  scales_of(t0, page0, ks0, vs0);
+  // plan u, waited for; the plans behind the last tile's stay unread
+  auto plan = [&](uint32_t u) -> const Plan & { return sh->plan[u % kPlans]; };
+  auto planned = [&](uint32_t u) { return warp_wait(p, &sh->plan_full[u % kPlans], u / kPlans & 1); };
+  bool more0 = planned(0) && plan(0).live != 0;
+  const bool early = !more0 || planned(1);
+  bool more1 = more0 && early && plan(1).live != 0;
+  if (!load_barrier(early)) return;  // all of them, or none
+  int page0 = more0 ? page_of(plan(0)) : kNone, page1 = more1 ? page_of(plan(1)) : kNone;
+  float ks0 = 0.f, vs0 = 0.f;
+  if (more0) scales_of(plan(0), page0, ks0, vs0);
   float value = 0.f;  // reference of V's scales
-  for (uint32_t used = 0; more0; ++used) {
+  uint32_t used = 0;
+  for (; more0; ++used) {
     const int stage = used % kStages, par = used & 1;
     const uint32_t phase = (used / kStages & 1) ^ 1;
-    const bool more2 = tiles.next(t2);
-    const int page2 = more2 ? page_of(t2) : kNone;
+    bool fine = !more1 || planned(used + 2);
+    const bool more2 = fine && more1 && plan(used + 2).live != 0;
+    const int page2 = more2 ? page_of(plan(used + 2)) : kNone;
     float ks1 = 0.f, vs1 = 0.f;
-    if (more1) scales_of(t1, page1, ks1, vs1);
+    if (more1) scales_of(plan(used + 1), page1, ks1, vs1);
+    const Plan &t0 = plan(used);
 
     int64_t off = -1;
     if (good(page0)) {
@@ -310,10 +325,14 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
     }
     load_barrier(true);
     float key = 1.f, move = 1.f;
-    if (t0.first) value = Q8 ? 0.f : 1.f;
+    if (t0.flags & kFirst) value = Q8 ? 0.f : 1.f;
     if (Q8) {
-      const float ktop = fmaxf(fmaxf(sh->top[par][0][0], sh->top[par][0][1]), fmaxf(sh->top[par][0][2], sh->top[par][0][3]));
-      const float vtop = fmaxf(fmaxf(sh->top[par][1][0], sh->top[par][1][1]), fmaxf(sh->top[par][1][2], sh->top[par][1][3]));
+      float ktop = 0.f, vtop = 0.f;
+#pragma unroll
+      for (int k = 0; k < KT / 32; ++k) {
+        ktop = fmaxf(ktop, sh->top[par][0][k]);
+        vtop = fmaxf(vtop, sh->top[par][1][k]);
+      }
       if (ktop > 0.f) key = ktop;
       if (vtop > value * kMaxRatio) {
         move = value / vtop;
@@ -346,7 +365,7 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
       }
     }
     // the stage's previous tile is used up, its description too
-    const bool fine = wait_or_report(p, &sh->k_empty[stage], phase) && wait_or_report(p, &sh->v_empty[stage], phase);
+    fine = fine && wait_or_report(p, &sh->k_empty[stage], phase) && wait_or_report(p, &sh->v_empty[stage], phase);
     TileInfo *info = &sh->tile[stage];
     if (tid == 0) {
       info->key = key;
@@ -354,12 +373,15 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
       info->value = value;
       info->base = t0.base;
       info->edge = edge;
+      info->live = t0.live;
+      info->last = t0.flags & kLast;
     }
     if (tid < KT / 32) {
       info->valid[tid] = sh->valid[par][tid];
       info->ghost[tid] = 0;
     }
     if (!load_barrier(fine)) break;
+    if (lane == 0) mbar_arrive(&sh->plan_empty[used % kPlans]);  // (every thread has read it)
 
     if (Q8) {
       auto convert = [&](int i, int r, int kv_i) {
@@ -426,8 +448,6 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
         }
       }
     }
-    t0 = t1;
-    t1 = t2;
     more0 = more1;
     more1 = more2;
     page0 = page1;
@@ -436,6 +456,56 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
     vs0 = vs1;
   }
   cp_async_wait_all();
+  // no more: an empty tile says so, in its turn
+  const uint32_t phase = (used / kStages & 1) ^ 1;
+  if (wait_or_report(p, &sh->k_empty[used % kStages], phase) && wait_or_report(p, &sh->v_empty[used % kStages], phase)) {
+    if (tid == 0) sh->tile[used % kStages].live = 0;
+    mbar_arrive(&sh->k_full[used % kStages]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Planning warp
+// ---------------------------------------------------------------------------
+template <int D>
+__device__ __forceinline__ void plan_tiles(const AttnParams &p, Shared *sh) {
+  constexpr int KT = Shape<D>::kKT;
+  const int lane = threadIdx.x & 31;
+  Walker<D> walker(p);
+  Item it{};
+  uint32_t items = 0, used = 0;
+  int64_t n = blockIdx.x;
+  for (;; ++items) {
+    const bool more = walker.seek(n, it);
+    if (!warp_wait(p, &sh->item_empty[items & 1], (items >> 1 & 1) ^ 1)) return;
+    if (lane == 0) {
+      sh->item[items & 1] = ItemInfo{more ? it.tiles : 0, it.seq.q0, it.seq.fresh, it.seq.total, it.head, it.row0, it.rows};
+      mbar_arrive(&sh->item_full[items & 1]);
+      if (more) n = static_cast<int64_t>(gridDim.x) + atomicAdd(p.items, 1);
+    }
+    n = __shfl_sync(0xffffffffu, n, 0);
+    const int live = more ? min(Shape<D>::kQTiles, (it.rows - it.row0 + 127) / 128) : 0;
+    for (int j = 0; j < (more ? it.tiles : 1); ++j, ++used) {
+      const int slot = used % kPlans;
+      if (!warp_wait(p, &sh->plan_empty[slot], (used / kPlans & 1) ^ 1)) return;
+      if (lane == 0) {
+        const bool in_head = j < it.head_tiles;
+        Plan t;
+        t.base = (in_head ? 0 : it.span.low) + (in_head ? j : j - it.head_tiles) * KT;
+        t.cnt = min(KT, (in_head ? it.span.head : it.span.end) - t.base);
+        t.e0 = it.seq.e0;
+        t.head = it.head;
+        t.first_pos = it.first_pos;
+        t.last_pos = it.last_pos;
+        t.live = live;
+        t.flags = (j == 0 ? kFirst : 0) | (j == it.tiles - 1 ? kLast : 0);
+        sh->plan[slot] = t;
+        mbar_arrive(&sh->plan_full[slot]);
+      }
+      __syncwarp();
+    }
+    if (!more) return;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -447,84 +517,106 @@ __device__ __forceinline__ void issue_products(const AttnParams &p, Shared *sh, 
   constexpr bool BF = std::is_same<T, Bf16>::value && !Q8;
   constexpr int KT = S::kKT;
   constexpr uint32_t kScores = f16_product(BF, 128, KT, false), kValues = f16_product(BF, 128, D, true);
-  const int lane = threadIdx.x & 31;
   const uint32_t tmem = sh->tmem, sq = smem_addr(q), skv = smem_addr(kv);
-  Walker<D> walker(p);
-  Item it;
-  uint32_t used = 0;
   uint32_t queries[2] = {0, 0}, weights[2] = {0, 0};  // waits on q_full and p_full so far
-  bool ok = true;
-  for (int64_t n = blockIdx.x; walker.seek(n, it); n += gridDim.x) {
-    const int live = min(S::kQTiles, (it.rows - it.row0 + 127) / 128);
-    if (lane == 0 && ok) {
-      auto scores = [&](int w, uint32_t tile) {
-        const uint32_t a = sq + w * S::kQBytes, b = skv + (tile % kStages) * 2 * S::kKVBytes;
+  // scores of a tile for row tile w; `done`: the last row tile's, K is used up
+  auto scores = [&](int w, uint32_t tile, bool done) {
+    const uint32_t a = sq + w * S::kQBytes, b = skv + (tile % kStages) * 2 * S::kKVBytes;
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-          mma_ss(tmem + S::kS + w * KT, tile_desc(a + (s / 4) * (128 * 128) + (s % 4) * 32, 16),
-                 tile_desc(b + (s / 4) * (KT * 128) + (s % 4) * 32, 16), kScores, s > 0);
-        mma_commit(&sh->s_full[w]);
-        if (w == live - 1) mma_commit(&sh->k_empty[tile % kStages]);
-      };
-      ok = wait_or_report(p, &sh->k_full[used % kStages], used / kStages & 1);
+    for (int s = 0; s < D / 16; ++s)
+      mma_ss(tmem + S::kS + w * KT, tile_desc(a + (s / 4) * (128 * 128) + (s % 4) * 32, 16),
+             tile_desc(b + (s / 4) * (KT * 128) + (s % 4) * 32, 16), kScores, s > 0);
+    mma_commit(&sh->s_full[w]);
+    if (done) mma_commit(&sh->k_empty[tile % kStages]);
+  };
+  bool first = true;
+  for (uint32_t tile = 0;; ++tile) {
+    const int stage = tile % kStages;
+    const uint32_t phase = tile / kStages & 1;
+    const TileInfo *info = &sh->tile[stage];
+    if (first) {  // of its item
+      if (!wait_or_report(p, &sh->k_full[stage], phase)) break;
+      const int live = info->live;
+      if (live == 0) break;
       fence_to_async();  // (asynchronous copies of a 16-bit pool arrive without one)
+      bool ok = true;
       for (int w = 0; w < live && ok; ++w) {
         ok = wait_or_report(p, &sh->q_full[w], queries[w]++ & 1);
         if (!ok) break;
         tc_fence_after();
-        scores(w, used);
+        scores(w, tile, w == live - 1);
       }
-      for (int j = 0; j < it.tiles && ok; ++j) {
-        const uint32_t tile = used + j;
-        ok = wait_or_report(p, &sh->v_full[tile % kStages], tile / kStages & 1);
-        fence_to_async();
-        for (int w = 0; w < live && ok; ++w) {
-          ok = wait_or_report(p, &sh->p_full[w], weights[w]++ & 1);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t b = skv + (tile % kStages) * 2 * S::kKVBytes + S::kKVBytes;
-#pragma unroll
-          for (int s = 0; s < KT / 16; ++s)
-            mma_ts(tmem + S::kO + w * D, tmem + S::kS + w * KT + s * 8, tile_desc(b + s * 2048, KT * 128), kValues,
-                   j > 0 || s > 0);
-          if (w == live - 1) mma_commit(&sh->v_empty[tile % kStages]);
-          if (j + 1 < it.tiles) {
-            if (w == 0) {
-              ok = wait_or_report(p, &sh->k_full[(tile + 1) % kStages], (tile + 1) / kStages & 1);
-              if (!ok) break;
-              fence_to_async();
-            }
-            scores(w, tile + 1);
-          } else {
-            mma_commit(&sh->o_full[w]);
-          }
-        }
-      }
+      if (!ok) break;
     }
-    used += it.tiles;
-    __syncwarp();
+    const int live = info->live;
+    const bool last = info->last != 0;
+    if (!wait_or_report(p, &sh->v_full[stage], phase)) break;
+    fence_to_async();
+    bool ok = true;
+    for (int w = 0; w < live && ok; ++w) {
+      ok = wait_or_report(p, &sh->p_full[w], weights[w]++ & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t b = skv + stage * 2 * S::kKVBytes + S::kKVBytes;
+#pragma unroll
+      for (int s = 0; s < KT / 16; ++s)
+        mma_ts(tmem + S::kO + w * D, tmem + S::kS + w * KT + s * 8, tile_desc(b + s * 2048, KT * 128), kValues,
+               !first || s > 0);
+      if (w == live - 1) mma_commit(&sh->v_empty[stage]);
+      if (last) {
+        mma_commit(&sh->o_full[w]);
+        continue;
+      }
+      if (w == 0) {
+        ok = wait_or_report(p, &sh->k_full[(tile + 1) % kStages], (tile + 1) / kStages & 1);
+        if (!ok) break;
+        fence_to_async();
+      }
+      scores(w, tile + 1, w == live - 1);
+    }
+    if (!ok) break;
+    first = last;
   }
-  if (lane == 0) {
-    // nothing of this CTA is in flight when its tensor memory goes
-    mma_commit(&sh->drained);
-    wait_or_report(p, &sh->drained, 0);
-  }
-  __syncwarp();
+  // nothing of this CTA is in flight when its tensor memory goes
+  mma_commit(&sh->drained);
+  wait_or_report(p, &sh->drained, 0);
 }
 
 // ---------------------------------------------------------------------------
-// Softmax warps: row tile w, one row per thread
+// Softmax warps: row tile w, half of the columns, one row per thread
 // ---------------------------------------------------------------------------
+// Pairs of floats in packed arithmetic.
+__device__ __forceinline__ uint64_t pair2(uint32_t a, uint32_t b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pack2(float a, float b) { return pair2(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // The lowest n bits, n of any sign.
 __device__ __forceinline__ uint32_t low_bits(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 }
 
-// This row's accumulator times a factor (rare: the reference of the weights moved).
-template <int D>
+// This half row's accumulator times a factor (rare: the reference of the weights
+// or of V's scales moved).
+template <int COLUMNS>
 __device__ __forceinline__ void rescale(uint32_t at, float factor) {
 #pragma unroll 1
-  for (int k = 0; k < D / 32; ++k) {
+  for (int k = 0; k < COLUMNS / 32; ++k) {
     uint32_t x[32];
     tmem_ld32(at + 32 * k, x);
 #pragma unroll
@@ -534,39 +626,50 @@ __device__ __forceinline__ void rescale(uint32_t at, float factor) {
 }
 
 template <typename T, int D, bool Q8>
-__device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, uint8_t *q, int w) {
+__device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, uint8_t *q, int w, int half) {
   using S = Shape<D>;
-  constexpr int KT = S::kKT;
+  constexpr int KT = S::kKT, C = KT / 2, DC = D / 2;  // columns of S and of O of this half
   constexpr bool BF = std::is_same<T, Bf16>::value && !Q8;
   constexpr float kLift = BF ? 0.f : 7.f;
   const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
   const int r = warp * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-  const uint32_t ts = sh->tmem + lanes + S::kS + w * KT, to = sh->tmem + lanes + S::kO + w * D;
+  const uint32_t ts = sh->tmem + lanes + S::kS + w * KT + half * C;      // scores of this half
+  const uint32_t tp = sh->tmem + lanes + S::kS + w * KT + half * C / 2;  // weights, two to a column
+  const uint32_t to = sh->tmem + lanes + S::kO + w * D + half * DC;
   const uint32_t sq = smem_addr(q) + w * S::kQBytes;
-  Walker<D> walker(p);
-  Item it;
+  float *mine = &sh->rows[w][half][r], *other = &sh->rows[w][half ^ 1][r];
   uint32_t used = 0, waits = 0, done = 0;
-  for (int64_t n = blockIdx.x; walker.seek(n, it); n += gridDim.x) {
+  // After a wait that gave up a thread waits no more, but meets its row tile's
+  // barriers until all of them leave together, at the next item.
+  bool lost = false;
+  auto wait = [&](uint64_t *bar, uint32_t parity) { lost = lost || !warp_wait(p, bar, parity); };
+  for (uint32_t items = 0;; ++items) {
+    wait(&sh->item_full[items & 1], items >> 1 & 1);
+    if (tile_barrier(w, lost)) return;
+    const ItemInfo it = sh->item[items & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh->item_empty[items & 1]);
+    if (it.tiles == 0) return;
     if (w >= S::kQTiles || it.row0 + w * 128 >= it.rows) {  // an item without this row tile
       used += it.tiles;
       continue;
     }
     const int row = it.row0 + w * 128 + r;
-    const int t = p.by_group.div(min(row, it.rows - 1)), g = min(row, it.rows - 1) - t * p.group;
-    const int64_t qrow = static_cast<int64_t>(it.seq.q0) + t;
+    const int t = p.by_group.div(min(row, it.rows - 1));
+    const int64_t qrow = static_cast<int64_t>(it.q0) + t;
     const bool has = row < it.rows && qrow < p.num_tokens;
-    const int pos = it.seq.total - it.seq.fresh + t;
-    const int64_t h = static_cast<int64_t>(it.head) * p.group + g;
+    const int pos = it.total - it.fresh + t;
+    const int64_t h = static_cast<int64_t>(it.head) * p.group + min(row, it.rows - 1) - t * p.group;
 
-    // this row's query, 16-bit and swizzled
+    // this row's query, 16-bit and swizzled, half of it
     float coef = p.scale_log2;
     {
       const uint4 *src = reinterpret_cast<const uint4 *>(p.q + (has ? qrow * p.q_row_stride + h * p.q_head_stride : 0));
       float up = 1.f;
       if (Q8 && std::is_same<T, Bf16>::value) {
         uint32_t big = 0;
-#pragma unroll 8
+#pragma unroll 4
         for (int c = 0; c < D / 8; ++c) {
           const uint4 x = has ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
           big = __vmaxu2(big, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
@@ -577,8 +680,9 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
         up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
         coef *= __uint_as_float(static_cast<uint32_t>(e) << 23);
       }
-#pragma unroll 8
-      for (int c = 0; c < D / 8; ++c) {
+#pragma unroll 4
+      for (int i = 0; i < D / 16; ++i) {
+        const int c = half * (D / 16) + i;
         uint4 x = has ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
         if (Q8 && std::is_same<T, Bf16>::value) {
           auto turn = [&](uint32_t &v) {
@@ -597,94 +701,111 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
       mbar_arrive(&sh->q_full[w]);
     }
 
-    float m = -INFINITY, l = 0.f, value = 1.f;
+    float m = -INFINITY, l = 0.f, value = 1.f;  // l: this half's sum
     for (int j = 0; j < it.tiles; ++j, ++used) {
       const int stage = used % kStages;
       const uint32_t phase = used / kStages & 1;
-      if (!warp_wait(p, &sh->s_full[w], waits++ & 1)) return;
-      if (!warp_wait(p, &sh->k_full[stage], phase)) return;  // (over: the description is the loading warps')
+      wait(&sh->s_full[w], waits++ & 1);
+      wait(&sh->k_full[stage], phase);  // (over: the description is the loading warps')
       tc_fence_after();
       const TileInfo *info = &sh->tile[stage];
       const float c = coef * info->key;
-      const float move = info->move;
+      float factor = info->move;
       const bool edge = info->edge != 0;
       value = info->value;
-      if (edge && !warp_wait(p, &sh->v_full[stage], phase)) return;  // which values were no numbers
-      // The scores in chunks of 64 columns: the maximum over all, the last chunk
-      // first; then the weights, the first chunk first (it is still in registers),
-      // each written over scores that are used up.
-      uint32_t x[64];
-      auto load = [&](int h) {
-        tmem_ld64(ts + 64 * h, x);
-        if (edge) {
-          // columns that this row sees: up to `last`, and past `out` or before `sink`
-          const int base = info->base + 64 * h;
-          const int last = pos - base + 1, out = p.window > 0 ? pos - p.window - base + 1 : 0;
-          const int sink = p.window > 0 ? p.sinks - base : 0;
+      if (edge) wait(&sh->v_full[stage], phase);  // which values were no numbers
+      auto hide = [&](uint32_t (&x)[32], int k) {  // the columns of chunk k that this row does not see
+        const int word = half * (C / 32) + k, base = info->base + 32 * word;
+        uint32_t see = info->valid[word] & low_bits(pos - base + 1);
+        if (p.window > 0) see &= ~low_bits(pos - p.window - base + 1) | low_bits(p.sinks - base);
+        const uint32_t ghost = info->ghost[word] & see;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t see =
-                info->valid[2 * h + k] & low_bits(last - 32 * k) & (~low_bits(out - 32 * k) | low_bits(sink - 32 * k));
-            const uint32_t ghost = info->ghost[2 * h + k] & see;
+        for (int i = 0; i < 32; ++i)
+          if (!((see >> i) & 1u)) x[i] = 0xff800000u;  // -inf
+        if (ghost) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((see >> i) & 1u)) x[32 * k + i] = 0xff800000u;  // -inf
-            if (ghost) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if ((ghost >> i) & 1u) x[32 * k + i] = 0x7fffffffu;  // NaN
-            }
-          }
+          for (int i = 0; i < 32; ++i)
+            if ((ghost >> i) & 1u) x[i] = 0x7fffffffu;  // NaN
         }
       };
-      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      uint32_t y[C / 2];  // the weights, not written before every thread of the row tile has read its scores
+      float sum;
+      const uint64_t c2 = pack2(c, c);
+      auto weigh = [&]() {
+        const float off = kLift - (m == -INFINITY ? 0.f : m);
+        const uint64_t off2 = pack2(off, off);
+        uint64_t sums[2] = {0, 0};
 #pragma unroll
-      for (int h = KT / 64 - 1; h >= 0; --h) {
-        load(h);
+        for (int k = 0; k < C / 32; ++k) {
+          uint32_t x[32];
+          tmem_ld32(ts + 32 * k, x);
+          if (edge) hide(x, k);
 #pragma unroll
-        for (int i = 0; i < 64; i += 8)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tops[k] = fmaxf(tops[k], fmaxf(__uint_as_float(x[i + 2 * k]), __uint_as_float(x[i + 2 * k + 1])));
-      }
-      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * c;
-      float factor = move;
-      if (top > m + kMoveBy) {
-        const float f = fast_exp2(m - top);
-        m = top;
-        l *= f;
-        factor *= f;
-      }
-      const bool moved = j > 0 && __any_sync(0xffffffffu, factor != 1.f);
-      const float off = kLift - (m == -INFINITY ? 0.f : m);
-      float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int h = 0; h < KT / 64; ++h) {
-        if (h > 0) load(h);
-        uint32_t y[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float a = fast_exp2(fmaf(__uint_as_float(x[2 * i]), c, off));
-          const float b = fast_exp2(fmaf(__uint_as_float(x[2 * i + 1]), c, off));
-          sums[2 * (i & 1)] += a;
-          sums[2 * (i & 1) + 1] += b;
-          y[i] = BF ? Bf16::pack(a, b) : Fp16::pack(a, b);
+          for (int i = 0; i < 16; ++i) {
+            float u, v;
+            unpack2(fma2(pair2(x[2 * i], x[2 * i + 1]), c2, off2), u, v);
+            u = fast_exp2(u);
+            v = fast_exp2(v);
+            sums[i & 1] = add2(sums[i & 1], pack2(u, v));
+            y[16 * k + i] = BF ? Bf16::pack(u, v) : Fp16::pack(u, v);
+          }
         }
-        tmem_st32(ts + 32 * h, y);
+        float s0, s1;
+        unpack2(add2(sums[0], sums[1]), s0, s1);
+        sum = s0 + s1;
+      };
+      // First with the reference as it stands: the sum of the weights tells whether
+      // any of them passes kMost, or is no number.
+      bool again = __any_sync(0xffffffffu, j == 0 || m == -INFINITY);
+      if (!again) {
+        weigh();
+        again = !(sum <= kMost);
       }
-      if (moved) rescale<D>(to, factor);
-      l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      if (tile_barrier(w, again)) {
+        // Else the maximum first; rows whose weights would pass 2^kMoveBy take it
+        // as their reference.
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int k = 0; k < C / 32; ++k) {
+          uint32_t x[32];
+          tmem_ld32(ts + 32 * k, x);
+          if (edge) hide(x, k);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
+        }
+        *mine = top;
+        tile_barrier(w, false);
+        top = fmaxf(top, *other) * c;
+        if (top > m + kMoveBy) {
+          const float f = fast_exp2(m - top);
+          m = top;
+          l *= f;
+          factor *= f;
+        }
+        weigh();
+        tile_barrier(w, false);  // before the first weight over scores, and before the next maximum
+      }
+      l += sum;
+      if constexpr (C == 64)
+        tmem_st32(tp, y);
+      else
+        tmem_st16(tp, y);
+      if (j > 0 && __any_sync(0xffffffffu, factor != 1.f)) rescale<DC>(to, factor);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&sh->p_full[w]);
     }
 
-    if (!warp_wait(p, &sh->o_full[w], done++ & 1)) return;
+    *mine = l;
+    tile_barrier(w, false);
+    l += *other;
+    wait(&sh->o_full[w], done++ & 1);
     tc_fence_after();
+    if (lost) continue;
     const float inv = l == 0.f ? 0.f : value / l;
-    char *out = p.o + (has ? qrow * p.o_row_stride + h * p.o_head_stride : 0);
+    char *out = p.o + (has ? qrow * p.o_row_stride + h * p.o_head_stride : 0) + half * DC * 2;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
+    for (int k = 0; k < DC / 32; ++k) {
       uint32_t x[32];
       tmem_ld32(to + 32 * k, x);
       if (has) {
@@ -717,34 +838,42 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
       mbar_init(&sh->v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh->q_full[i], 128);
+      mbar_init(&sh->q_full[i], kTileThreads);
       mbar_init(&sh->s_full[i], 1);
-      mbar_init(&sh->p_full[i], 128);
+      mbar_init(&sh->p_full[i], kTileThreads);
+      mbar_init(&sh->item_full[i], 1);
+      mbar_init(&sh->item_empty[i], kSoftmaxWarps);
+      mbar_init(&sh->plan_full[2 * i], 1);
+      mbar_init(&sh->plan_full[2 * i + 1], 1);
+      mbar_init(&sh->plan_empty[2 * i], kLoadWarps);
+      mbar_init(&sh->plan_empty[2 * i + 1], kLoadWarps);
       mbar_init(&sh->o_full[i], 1);
     }
     mbar_init(&sh->drained, 1);
     fence_mbar_init();
   }
-  if (warp == 12) tmem_alloc(&sh->tmem, 512);
+  if (warp == kThreads / 32 - 4) tmem_alloc(&sh->tmem, 512);
   pdl_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // registers of the launch (512 x 128) shared out by role: 256 x 152 + 128 x 112 + 128 x 96
-  if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
-    softmax_rows<T, D, Q8>(p, sh, q, warp >> 2);
-  } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+  // registers of the launch (896 x 72) shared out by role: 512 x 88 + 256 x 56 + 128 x 40
+  if (warp < kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    softmax_rows<T, D, Q8>(p, sh, q, warp >> 3, warp >> 2 & 1);
+  } else if (warp < kSoftmaxWarps + kLoadWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     load_tiles<T, D, Q8>(p, sh, kv);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-    if (warp == 12) issue_products<T, D, Q8>(p, sh, q, kv);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == kThreads / 32 - 3) plan_tiles<D>(p, sh);
+    if (threadIdx.x == kThreads - 128) issue_products<T, D, Q8>(p, sh, q, kv);
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_free(sh->tmem, 512);
+  if (warp == kThreads / 32 - 4) tmem_free(sh->tmem, 512);
 }
 
 }  // namespace

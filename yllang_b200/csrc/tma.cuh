@@ -70,6 +70,17 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity
   return true;
 }
 
+// The same bound by the SM's clock, 2^32 cycles (2 s and more), for waits on a
+// kernel's critical path: reading it costs little beside %globaltimer.
+__device__ __forceinline__ bool mbar_wait_clocked(uint64_t *bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (clock64() - t0 > (1ll << 32)) return false;
+  }
+  return true;
+}
+
 // global -> shared, completing `bytes` on `bar`.
 __device__ __forceinline__ void bulk_load(void *smem_dst, const void *gmem_src, uint32_t bytes, uint64_t *bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
