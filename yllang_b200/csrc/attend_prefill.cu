@@ -27,7 +27,7 @@
 //   read S once and write the weights over it in 16 bits.  The weights refer to
 //   an earlier tile's maximum: that is looked at again, and the row's accumulator
 //   rescaled, only where a sum of weights shows that one may have grown past
-//   2^8 (fp16 weights are kept times 2^7).
+//   2^8 (fp16 weights are kept times 2^3).
 //
 // Only tiles that some row does not see in full are masked; in those, infinities
 // and NaN of V are zeroed as they are loaded and reported to the rows that see
@@ -47,7 +47,8 @@ constexpr int kSoftmaxWarps = 16, kLoadWarps = 8;
 constexpr int kThreads = (kSoftmaxWarps + kLoadWarps + 4) * 32;
 constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int kTileThreads = 256;  // softmax threads of a row tile
-constexpr int kStages = 2;
+constexpr int kStages = 2;  // of K, and of V
+constexpr int kInfos = 4;   // descriptions of tiles: one is read until the tile's values are used up
 constexpr float kMoveBy = 8.f;    // log2 of how far weights may pass 1 before their reference moves
 constexpr float kMost = 32768.f;  // sum of weights of half a row, lift included, above which they are looked at again
 constexpr float kMaxRatio = 64.f; // of a V scale to the reference
@@ -102,7 +103,7 @@ struct Shared {
   uint32_t tmem;
   float top[2][2][kLoadWarps];     // [parity][K, V][loading warp]: largest scales
   uint32_t valid[2][4];            // [parity]: tokens with a good page
-  TileInfo tile[kStages];
+  TileInfo tile[kInfos];
   ItemInfo item[2];
   Plan plan[kPlans];
   int64_t offset[2][128];          // [parity]: byte offset of a token's head row
@@ -288,6 +289,7 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
   float ks0 = 0.f, vs0 = 0.f;
   if (more0) scales_of(plan(0), page0, ks0, vs0);
   float value = 0.f;  // reference of V's scales
+  bool lost = false;  // a wait gave up: the next barrier ends all of them
   uint32_t used = 0;
   for (; more0; ++used) {
     const int stage = used % kStages, par = used & 1;
@@ -364,9 +366,9 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
         if (o >= 0) w[i] = __ldg(reinterpret_cast<const uint4 *>(p.kv[0] + o + c * 16));
       }
     }
-    // the stage's previous tile is used up, its description too
-    fine = fine && wait_or_report(p, &sh->k_empty[stage], phase) && wait_or_report(p, &sh->v_empty[stage], phase);
-    TileInfo *info = &sh->tile[stage];
+    // K's previous tile of this stage is used up; V's is waited for behind K
+    fine = fine && !lost && wait_or_report(p, &sh->k_empty[stage], phase);
+    TileInfo *info = &sh->tile[used % kInfos];
     if (tid == 0) {
       info->key = key;
       info->move = move;
@@ -413,6 +415,7 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
       }
       fence_to_async();
       mbar_arrive(&sh->k_full[stage]);
+      lost = !wait_or_report(p, &sh->v_empty[stage], phase);
 #pragma unroll
       for (int i = 0; i < PER; ++i) convert(i, r0 + i * STEP, 1);
       fence_to_async();
@@ -420,6 +423,7 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
     } else {
 #pragma unroll
       for (int kv_i = 0; kv_i < 2; ++kv_i) {
+        if (kv_i == 1) lost = !wait_or_report(p, &sh->v_empty[stage], phase);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int r = r0 + i * STEP;
@@ -457,9 +461,8 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
   }
   cp_async_wait_all();
   // no more: an empty tile says so, in its turn
-  const uint32_t phase = (used / kStages & 1) ^ 1;
-  if (wait_or_report(p, &sh->k_empty[used % kStages], phase) && wait_or_report(p, &sh->v_empty[used % kStages], phase)) {
-    if (tid == 0) sh->tile[used % kStages].live = 0;
+  if (wait_or_report(p, &sh->k_empty[used % kStages], (used / kStages & 1) ^ 1)) {
+    if (tid == 0) sh->tile[used % kInfos].live = 0;
     mbar_arrive(&sh->k_full[used % kStages]);
   }
 }
@@ -509,7 +512,7 @@ __device__ __forceinline__ void plan_tiles(const AttnParams &p, Shared *sh) {
 }
 
 // ---------------------------------------------------------------------------
-// Product warp (one thread)
+// Product warp
 // ---------------------------------------------------------------------------
 template <typename T, int D, bool Q8>
 __device__ __forceinline__ void issue_products(const AttnParams &p, Shared *sh, uint8_t *q, uint8_t *kv) {
@@ -521,27 +524,31 @@ __device__ __forceinline__ void issue_products(const AttnParams &p, Shared *sh, 
   uint32_t queries[2] = {0, 0}, weights[2] = {0, 0};  // waits on q_full and p_full so far
   // scores of a tile for row tile w; `done`: the last row tile's, K is used up
   auto scores = [&](int w, uint32_t tile, bool done) {
-    const uint32_t a = sq + w * S::kQBytes, b = skv + (tile % kStages) * 2 * S::kKVBytes;
+    const uint64_t a = tile_desc(sq + w * S::kQBytes, 16);
+    const uint64_t b = tile_desc(skv + (tile % kStages) * 2 * S::kKVBytes, 16);
+    if (elect_one()) {
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s)
-      mma_ss(tmem + S::kS + w * KT, tile_desc(a + (s / 4) * (128 * 128) + (s % 4) * 32, 16),
-             tile_desc(b + (s / 4) * (KT * 128) + (s % 4) * 32, 16), kScores, s > 0);
-    mma_commit(&sh->s_full[w]);
-    if (done) mma_commit(&sh->k_empty[tile % kStages]);
+      for (int s = 0; s < D / 16; ++s)  // (addresses count in 16 bytes)
+        mma_ss(tmem + S::kS + w * KT, a + ((s / 4) * (128 * 128) + (s % 4) * 32) / 16,
+               b + ((s / 4) * (KT * 128) + (s % 4) * 32) / 16, kScores, s > 0);
+      mma_commit(&sh->s_full[w]);
+      if (done) mma_commit(&sh->k_empty[tile % kStages]);
+    }
+    __syncwarp();
   };
   bool first = true;
   for (uint32_t tile = 0;; ++tile) {
     const int stage = tile % kStages;
     const uint32_t phase = tile / kStages & 1;
-    const TileInfo *info = &sh->tile[stage];
+    const TileInfo *info = &sh->tile[tile % kInfos];
     if (first) {  // of its item
-      if (!wait_or_report(p, &sh->k_full[stage], phase)) break;
+      if (!warp_wait(p, &sh->k_full[stage], phase)) break;
       const int live = info->live;
       if (live == 0) break;
       fence_to_async();  // (asynchronous copies of a 16-bit pool arrive without one)
       bool ok = true;
       for (int w = 0; w < live && ok; ++w) {
-        ok = wait_or_report(p, &sh->q_full[w], queries[w]++ & 1);
+        ok = warp_wait(p, &sh->q_full[w], queries[w]++ & 1);
         if (!ok) break;
         tc_fence_after();
         scores(w, tile, w == live - 1);
@@ -550,36 +557,33 @@ __device__ __forceinline__ void issue_products(const AttnParams &p, Shared *sh, 
     }
     const int live = info->live;
     const bool last = info->last != 0;
-    if (!wait_or_report(p, &sh->v_full[stage], phase)) break;
+    if (!warp_wait(p, &sh->v_full[stage], phase)) break;
+    if (!last && !warp_wait(p, &sh->k_full[(tile + 1) % kStages], (tile + 1) / kStages & 1)) break;
     fence_to_async();
     bool ok = true;
     for (int w = 0; w < live && ok; ++w) {
-      ok = wait_or_report(p, &sh->p_full[w], weights[w]++ & 1);
+      ok = warp_wait(p, &sh->p_full[w], weights[w]++ & 1);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t b = skv + stage * 2 * S::kKVBytes + S::kKVBytes;
+      const uint64_t b = tile_desc(skv + stage * 2 * S::kKVBytes + S::kKVBytes, KT * 128);
+      if (elect_one()) {
 #pragma unroll
-      for (int s = 0; s < KT / 16; ++s)
-        mma_ts(tmem + S::kO + w * D, tmem + S::kS + w * KT + s * 8, tile_desc(b + s * 2048, KT * 128), kValues,
-               !first || s > 0);
-      if (w == live - 1) mma_commit(&sh->v_empty[stage]);
-      if (last) {
-        mma_commit(&sh->o_full[w]);
-        continue;
+        for (int s = 0; s < KT / 16; ++s)
+          mma_ts(tmem + S::kO + w * D, tmem + S::kS + w * KT + s * 8, b + s * (2048 / 16), kValues, !first || s > 0);
+        if (w == live - 1) mma_commit(&sh->v_empty[stage]);
+        if (last) mma_commit(&sh->o_full[w]);
       }
-      if (w == 0) {
-        ok = wait_or_report(p, &sh->k_full[(tile + 1) % kStages], (tile + 1) / kStages & 1);
-        if (!ok) break;
-        fence_to_async();
-      }
+      __syncwarp();
+      if (last) continue;
       scores(w, tile + 1, w == live - 1);
     }
     if (!ok) break;
     first = last;
   }
   // nothing of this CTA is in flight when its tensor memory goes
-  mma_commit(&sh->drained);
-  wait_or_report(p, &sh->drained, 0);
+  if (elect_one()) mma_commit(&sh->drained);
+  __syncwarp();
+  warp_wait(p, &sh->drained, 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -630,7 +634,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
   using S = Shape<D>;
   constexpr int KT = S::kKT, C = KT / 2, DC = D / 2;  // columns of S and of O of this half
   constexpr bool BF = std::is_same<T, Bf16>::value && !Q8;
-  constexpr float kLift = BF ? 0.f : 7.f;
+  constexpr float kLift = BF ? 0.f : 3.f;
   const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
   const int r = warp * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
@@ -706,9 +710,8 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
       const int stage = used % kStages;
       const uint32_t phase = used / kStages & 1;
       wait(&sh->s_full[w], waits++ & 1);
-      wait(&sh->k_full[stage], phase);  // (over: the description is the loading warps')
       tc_fence_after();
-      const TileInfo *info = &sh->tile[stage];
+      const TileInfo *info = &sh->tile[used % kInfos];
       const float c = coef * info->key;
       float factor = info->move;
       const bool edge = info->edge != 0;
@@ -867,8 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == kThreads / 32 - 3) plan_tiles<D>(p, sh);
-    if (threadIdx.x == kThreads - 128) issue_products<T, D, Q8>(p, sh, q, kv);
-    __syncwarp();
+    if (warp == kThreads / 32 - 4) issue_products<T, D, Q8>(p, sh, q, kv);
   }
   tc_fence_before();
   __syncthreads();
