@@ -487,6 +487,15 @@ __device__ __forceinline__ void plan_tiles(const AttnParams &p, Shared *sh) {
       if (more) n = static_cast<int64_t>(gridDim.x) + atomicAdd(p.items, 1);
     }
     n = __shfl_sync(0xffffffffu, n, 0);
+    // its queries on their way into the L2 cache
+    if (more)
+      for (int i = lane; i < Shape<D>::kRows * (D / 64); i += 32) {
+        const int row = it.row0 + i / (D / 64), t = p.by_group.div(row);
+        if (row < it.rows && it.seq.q0 + static_cast<int64_t>(t) < p.num_tokens)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(
+              p.q + (it.seq.q0 + static_cast<int64_t>(t)) * p.q_row_stride +
+              (static_cast<int64_t>(it.head) * p.group + (row - t * p.group)) * p.q_head_stride + i % (D / 64) * 128));
+      }
     const int live = more ? min(Shape<D>::kQTiles, (it.rows - it.row0 + 127) / 128) : 0;
     for (int j = 0; j < (more ? it.tiles : 1); ++j, ++used) {
       const int slot = used % kPlans;
@@ -659,77 +668,91 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
       used += it.tiles;
       continue;
     }
-    const int row = it.row0 + w * 128 + r;
-    const int t = p.by_group.div(min(row, it.rows - 1));
-    const int64_t qrow = static_cast<int64_t>(it.q0) + t;
-    const bool has = row < it.rows && qrow < p.num_tokens;
-    const int pos = it.total - it.fresh + t;
-    const int64_t h = static_cast<int64_t>(it.head) * p.group + min(row, it.rows - 1) - t * p.group;
-
-    // this row's query, 16-bit and swizzled, half of it
+    const int pos = it.total - it.fresh + static_cast<int>(p.by_group.div(min(it.row0 + w * 128 + r, it.rows - 1)));
+    // Rows move between global and shared memory in whole: 16-byte chunk
+    // `chunk` of rows r0, r0 + STEP, .. is this thread's.
+    constexpr int CH = D / 8, STEP = kTileThreads / CH, PER = 128 / STEP;
+    const int tid = threadIdx.x & (kTileThreads - 1), chunk = tid % CH, r0 = tid / CH;
+    // byte offset of row i of the row tile in a tensor of these strides; -1: no such row
+    auto row_at = [&](int i, int64_t row_stride, int64_t head_stride) -> int64_t {
+      const int row = it.row0 + w * 128 + i;
+      const int t = p.by_group.div(row);
+      if (row >= it.rows || it.q0 + static_cast<int64_t>(t) >= p.num_tokens) return -1;
+      return (it.q0 + static_cast<int64_t>(t)) * row_stride +
+             (static_cast<int64_t>(it.head) * p.group + (row - t * p.group)) * head_stride;
+    };
+    // the queries, 16-bit and swizzled
     float coef = p.scale_log2;
     {
-      const uint4 *src = reinterpret_cast<const uint4 *>(p.q + (has ? qrow * p.q_row_stride + h * p.q_head_stride : 0));
-      float up = 1.f;
-      if (Q8 && std::is_same<T, Bf16>::value) {
-        uint32_t big = 0;
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 x = has ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-          big = __vmaxu2(big, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
-                                       __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
-        }
-        big = max(big & 0xffffu, big >> 16);
-        const int e = min(max(static_cast<int>(big >> 7), 1), 253);  // biased exponent of the largest element
-        up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-        coef *= __uint_as_float(static_cast<uint32_t>(e) << 23);
+      uint4 x[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int64_t at = row_at(r0 + i * STEP, p.q_row_stride, p.q_head_stride);
+        x[i] = at >= 0 ? __ldg(reinterpret_cast<const uint4 *>(p.q + at) + chunk) : make_uint4(0, 0, 0, 0);
       }
-#pragma unroll 4
-      for (int i = 0; i < D / 16; ++i) {
-        const int c = half * (D / 16) + i;
-        uint4 x = has ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int row = r0 + i * STEP;
         if (Q8 && std::is_same<T, Bf16>::value) {
+          uint32_t big = __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu),
+                                  __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
+#pragma unroll
+          for (int d = CH / 2; d > 0; d >>= 1) big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, d));
+          big = max(big & 0xffffu, big >> 16);
+          const int e = min(max(static_cast<int>(big >> 7), 1), 253);  // biased exponent of the row's largest element
+          const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+          if (chunk == 0) sh->rows[w][0][row] = __uint_as_float(static_cast<uint32_t>(e) << 23);
           auto turn = [&](uint32_t &v) {
             const float2 f = Bf16::unpack(v);
             v = Fp16::pack(f.x * up, f.y * up);
           };
-          turn(x.x);
-          turn(x.y);
-          turn(x.z);
-          turn(x.w);
+          turn(x[i].x);
+          turn(x[i].y);
+          turn(x[i].z);
+          turn(x[i].w);
         }
-        sts128(sq + swizzled<128>(r, c), x.x, x.y, x.z, x.w);
+        sts128(sq + swizzled<128>(row, chunk), x[i].x, x[i].y, x[i].z, x[i].w);
       }
       fence_to_async();
       tc_fence_before();  // the previous item's accumulators are read
       mbar_arrive(&sh->q_full[w]);
+      if (Q8 && std::is_same<T, Bf16>::value) {
+        tile_barrier(w, false);
+        coef *= sh->rows[w][0][r];
+        tile_barrier(w, false);  // before the array's next use
+      }
     }
 
+    // the columns of word k of a tile that this row sees
+    auto seen = [&](const TileInfo *info, int word) {
+      const int base = info->base + 32 * word;
+      uint32_t see = info->valid[word] & low_bits(pos - base + 1);
+      if (p.window > 0) see &= ~low_bits(pos - p.window - base + 1) | low_bits(p.sinks - base);
+      return see;
+    };
+    bool ghostly = false;  // a value that this row sees was no number
+    auto look_back = [&](uint32_t tile) {  // at an edge tile whose values are loaded by now
+      const TileInfo *info = &sh->tile[tile % kInfos];
+#pragma unroll
+      for (int k = 0; k < C / 32; ++k)
+        if (info->ghost[half * (C / 32) + k] & seen(info, half * (C / 32) + k)) ghostly = true;
+    };
+    bool edge = false;
     float m = -INFINITY, l = 0.f, value = 1.f;  // l: this half's sum
     for (int j = 0; j < it.tiles; ++j, ++used) {
-      const int stage = used % kStages;
-      const uint32_t phase = used / kStages & 1;
-      wait(&sh->s_full[w], waits++ & 1);
+      wait(&sh->s_full[w], waits++ & 1);  // (issued behind the tile's description)
       tc_fence_after();
       const TileInfo *info = &sh->tile[used % kInfos];
       const float c = coef * info->key;
       float factor = info->move;
-      const bool edge = info->edge != 0;
+      if (edge) look_back(used - 1);  // (the scores' products were issued behind its values')
+      edge = info->edge != 0;
       value = info->value;
-      if (edge) wait(&sh->v_full[stage], phase);  // which values were no numbers
       auto hide = [&](uint32_t (&x)[32], int k) {  // the columns of chunk k that this row does not see
-        const int word = half * (C / 32) + k, base = info->base + 32 * word;
-        uint32_t see = info->valid[word] & low_bits(pos - base + 1);
-        if (p.window > 0) see &= ~low_bits(pos - p.window - base + 1) | low_bits(p.sinks - base);
-        const uint32_t ghost = info->ghost[word] & see;
+        const uint32_t see = seen(info, half * (C / 32) + k);
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (!((see >> i) & 1u)) x[i] = 0xff800000u;  // -inf
-        if (ghost) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if ((ghost >> i) & 1u) x[i] = 0x7fffffffu;  // NaN
-        }
+          if (!(see & (1u << i))) x[i] = 0xff800000u;  // -inf
       };
       uint32_t y[C / 2];  // the weights, not written before every thread of the row tile has read its scores
       float sum;
@@ -799,28 +822,37 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
       mbar_arrive(&sh->p_full[w]);
     }
 
-    *mine = l;
-    tile_barrier(w, false);
-    l += *other;
     wait(&sh->o_full[w], done++ & 1);
     tc_fence_after();
-    if (lost) continue;
+    if (edge) look_back(used - 1);
+    *mine = ghostly ? NAN : l;
+    tile_barrier(w, false);
+    l = (ghostly ? NAN : l) + *other;
     const float inv = l == 0.f ? 0.f : value / l;
-    char *out = p.o + (has ? qrow * p.o_row_stride + h * p.o_head_stride : 0) + half * DC * 2;
+    // through the shared memory of the queries, which are used up
 #pragma unroll
     for (int k = 0; k < DC / 32; ++k) {
       uint32_t x[32];
       tmem_ld32(to + 32 * k, x);
-      if (has) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          uint32_t y[4];
+      for (int i = 0; i < 32; i += 8) {
+        uint32_t y[4];
 #pragma unroll
-          for (int a = 0; a < 4; ++a)
-            y[a] = T::pack(__uint_as_float(x[i + 2 * a]) * inv, __uint_as_float(x[i + 2 * a + 1]) * inv);
-          *reinterpret_cast<uint4 *>(out + (32 * k + i) * 2) = make_uint4(y[0], y[1], y[2], y[3]);
-        }
+        for (int a = 0; a < 4; ++a)
+          y[a] = T::pack(__uint_as_float(x[i + 2 * a]) * inv, __uint_as_float(x[i + 2 * a + 1]) * inv);
+        sts128(sq + swizzled<128>(r, half * (DC / 8) + 4 * k + i / 8), y[0], y[1], y[2], y[3]);
       }
+    }
+    tile_barrier(w, false);
+    if (lost) continue;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int64_t at = row_at(r0 + i * STEP, p.o_row_stride, p.o_head_stride);
+      uint32_t y[4];
+      asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3])
+                   : "r"(sq + swizzled<128>(r0 + i * STEP, chunk)));
+      if (at >= 0) *(reinterpret_cast<uint4 *>(p.o + at) + chunk) = make_uint4(y[0], y[1], y[2], y[3]);
     }
   }
 }
