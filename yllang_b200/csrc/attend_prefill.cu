@@ -53,6 +53,8 @@ constexpr float kMoveBy = 8.f;    // log2 of how far weights may pass 1 before t
 constexpr float kMost = 32768.f;  // sum of weights of half a row, lift included, above which they are looked at again
 constexpr float kMaxRatio = 64.f; // of a V scale to the reference
 
+constexpr int kHeader = 12288;  // bytes of Shared
+
 template <int D>
 struct Shape {
   static constexpr int kQTiles = D == 256 ? 1 : 2;  // 128-row tiles of an item
@@ -60,7 +62,7 @@ struct Shape {
   static constexpr int kRows = 128 * kQTiles;
   static constexpr int kQBytes = 128 * D * 2;       // one row tile
   static constexpr int kKVBytes = kKT * D * 2;      // K or V of a stage
-  static constexpr int kSmem = kQTiles * kQBytes + 2 * kStages * kKVBytes + 8192 + 1024;
+  static constexpr int kSmem = kQTiles * kQBytes + 2 * kStages * kKVBytes + kHeader + 1024;
   static constexpr uint32_t kS = 0;    // tensor memory columns: S of tile w at w * kKT
   static constexpr uint32_t kO = 256;  // O of tile w at kO + w * D
 };
@@ -109,8 +111,9 @@ struct Shared {
   int64_t offset[2][128];          // [parity]: byte offset of a token's head row
   uint32_t ratio[2][2][128];       // [parity][K, V]: scale over the reference, two halves
   float rows[2][2][128];           // [row tile][half of the columns]: a row's maximum or sum
+  int64_t row_at[2][2][128];       // [row tile][q, o]: byte offset of a row, -1 for none
 };
-static_assert(sizeof(Shared) <= 8192, "shared header");
+static_assert(sizeof(Shared) <= kHeader, "shared header");
 
 struct Item {
   Seq seq;
@@ -673,46 +676,52 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
     // `chunk` of rows r0, r0 + STEP, .. is this thread's.
     constexpr int CH = D / 8, STEP = kTileThreads / CH, PER = 128 / STEP;
     const int tid = threadIdx.x & (kTileThreads - 1), chunk = tid % CH, r0 = tid / CH;
-    // byte offset of row i of the row tile in a tensor of these strides; -1: no such row
-    auto row_at = [&](int i, int64_t row_stride, int64_t head_stride) -> int64_t {
-      const int row = it.row0 + w * 128 + i;
-      const int t = p.by_group.div(row);
-      if (row >= it.rows || it.q0 + static_cast<int64_t>(t) >= p.num_tokens) return -1;
-      return (it.q0 + static_cast<int64_t>(t)) * row_stride +
-             (static_cast<int64_t>(it.head) * p.group + (row - t * p.group)) * head_stride;
-    };
+    {  // their places: row r of the row tile in q (half 0) or o (half 1)
+      const int row = it.row0 + w * 128 + r, t = p.by_group.div(row);
+      const int64_t token = it.q0 + static_cast<int64_t>(t), head = static_cast<int64_t>(it.head) * p.group + (row - t * p.group);
+      const bool has = row < it.rows && token < p.num_tokens;
+      sh->row_at[w][half][r] = !has ? -1 : half ? token * p.o_row_stride + head * p.o_head_stride
+                                                : token * p.q_row_stride + head * p.q_head_stride;
+    }
+    tile_barrier(w, false);
     // the queries, 16-bit and swizzled
     float coef = p.scale_log2;
     {
       uint4 x[PER];
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int64_t at = row_at(r0 + i * STEP, p.q_row_stride, p.q_head_stride);
+        const int64_t at = sh->row_at[w][0][r0 + i * STEP];
         x[i] = at >= 0 ? __ldg(reinterpret_cast<const uint4 *>(p.q + at) + chunk) : make_uint4(0, 0, 0, 0);
       }
+      if (Q8 && std::is_same<T, Bf16>::value) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int row = r0 + i * STEP;
-        if (Q8 && std::is_same<T, Bf16>::value) {
-          uint32_t big = __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu),
-                                  __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
+        for (int i = 0; i < PER; i += 2) {  // two rows' largest elements in one word
+          auto largest = [](const uint4 &v) {
+            const uint32_t b = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                        __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+            return max(b & 0xffffu, b >> 16);
+          };
+          uint32_t big = largest(x[i]) | largest(x[i + 1]) << 16;
 #pragma unroll
           for (int d = CH / 2; d > 0; d >>= 1) big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, d));
-          big = max(big & 0xffffu, big >> 16);
-          const int e = min(max(static_cast<int>(big >> 7), 1), 253);  // biased exponent of the row's largest element
-          const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-          if (chunk == 0) sh->rows[w][0][row] = __uint_as_float(static_cast<uint32_t>(e) << 23);
-          auto turn = [&](uint32_t &v) {
-            const float2 f = Bf16::unpack(v);
-            v = Fp16::pack(f.x * up, f.y * up);
-          };
-          turn(x[i].x);
-          turn(x[i].y);
-          turn(x[i].z);
-          turn(x[i].w);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int e = min(max(static_cast<int>((k ? big >> 16 : big & 0xffffu) >> 7), 1), 253);  // biased exponent
+            const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+            if (chunk == 0) sh->rows[w][0][r0 + (i + k) * STEP] = __uint_as_float(static_cast<uint32_t>(e) << 23);
+            auto turn = [&](uint32_t &v) {
+              const float2 f = Bf16::unpack(v);
+              v = Fp16::pack(f.x * up, f.y * up);
+            };
+            turn(x[i + k].x);
+            turn(x[i + k].y);
+            turn(x[i + k].z);
+            turn(x[i + k].w);
+          }
         }
-        sts128(sq + swizzled<128>(row, chunk), x[i].x, x[i].y, x[i].z, x[i].w);
       }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sts128(sq + swizzled<128>(r0 + i * STEP, chunk), x[i].x, x[i].y, x[i].z, x[i].w);
       fence_to_async();
       tc_fence_before();  // the previous item's accumulators are read
       mbar_arrive(&sh->q_full[w]);
@@ -782,22 +791,29 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
       };
       // First with the reference as it stands: the sum of the weights tells whether
       // any of them passes kMost, or is no number.
-      bool again = __any_sync(0xffffffffu, j == 0 || m == -INFINITY);
+      bool again = j == 0;
       if (!again) {
-        weigh();
-        again = !(sum <= kMost);
+        again = __any_sync(0xffffffffu, m == -INFINITY);
+        if (!again) {
+          weigh();
+          again = !(sum <= kMost);
+        }
+        again = tile_barrier(w, again);
       }
-      if (tile_barrier(w, again)) {
-        // Else the maximum first; rows whose weights would pass 2^kMoveBy take it
-        // as their reference.
+      if (again) {
+        // Else, and for the first tile, the maximum first; rows whose weights would
+        // pass 2^kMoveBy take it as their reference.
         float top = -INFINITY;
-#pragma unroll 1
+#pragma unroll
         for (int k = 0; k < C / 32; ++k) {
           uint32_t x[32];
           tmem_ld32(ts + 32 * k, x);
           if (edge) hide(x, k);
+          float tops[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
+          for (int i = 0; i < 16; ++i)
+            tops[i & 1] = fmaxf(tops[i & 1], fmaxf(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])));
+          top = fmaxf(top, fmaxf(tops[0], tops[1]));
         }
         *mine = top;
         tile_barrier(w, false);
@@ -847,7 +863,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
     if (lost) continue;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int64_t at = row_at(r0 + i * STEP, p.o_row_stride, p.o_head_stride);
+      const int64_t at = sh->row_at[w][1][r0 + i * STEP];
       uint32_t y[4];
       asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                    : "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3])
