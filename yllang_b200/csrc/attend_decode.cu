@@ -11,10 +11,11 @@
 //   place by scanning the batch itself (a few KB), so a call needs no plan.
 //   A (sequence, head) whose units fall in several CTAs leaves its parts in the
 //   workspace, and a second kernel joins them, in a fixed order.
-// * One warp of a CTA only issues loads: it walks the units, looks up pages one
-//   unit ahead, and fills a ring of stages with 16-byte asynchronous copies,
-//   across the ends of sequences.  Tokens that no query sees are zero-filled,
-//   not read.
+// * Four warps of a CTA only issue loads, a quarter of a unit's tokens each: they
+//   walk the units, look up pages one unit ahead, and fill a ring of stages with
+//   16-byte asynchronous copies, across the ends of sequences.  (One such warp
+//   spent 3,300 cycles on a unit whose bytes HBM delivers in 1,500.)  Tokens that
+//   no query sees are zero-filled, not read.
 // * Four warps compute, each on its own quarter of the tile with its own running
 //   maximum, sum and accumulator (online softmax); the four are joined when a
 //   (sequence, head) ends.  Products are m16n8k16 matrix instructions with the
@@ -46,14 +47,14 @@ namespace ylk {
 namespace {
 
 constexpr int kConsumers = 4;  // warps that compute, a quarter of a unit's tokens each
-constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int kThreads = 2 * kConsumers * 32;  // and as many that load
 // A CTA's run is at least this many units, so that a short sequence is not cut
 // into parts whose joining costs more than they save.
 constexpr int kMinRun = 2;
 
-// Unit descriptor in a stage, written by the loading warp.
+// Unit descriptor in a stage, written by the loading warps.
 struct UnitInfo {
-  uint32_t valid[4];  // tokens of the tile that some query sees, with a good page
+  uint32_t valid[4];  // of a quarter of the tile: tokens that some query sees, with a good page
   int base;           // position of the tile's first token
   int flags;          // kFirst | kLast | kWhole | kRagged
   int pos0;           // position of the sequence's first query
@@ -262,46 +263,40 @@ __device__ __forceinline__ bool find_place(const AttnParams &p, Place &out) {
 }
 
 // ---------------------------------------------------------------------------
-// Loading warp
+// Loading warps
 // ---------------------------------------------------------------------------
 template <int D, bool Q8, int NB>
 __device__ __forceinline__ void load_units(const AttnParams &p, const Place &place, uint8_t *stages, uint64_t *full,
                                            uint64_t *empty) {
   using L = Layout<D, Q8, NB>;
-  constexpr int kTile = L::kTile, kRows = L::kRows, KT = kTile / 32;  // tokens of a lane
-  const int lane = threadIdx.x & 31;
+  constexpr int kTile = L::kTile, kRows = L::kRows, kTokens = L::kTokens;  // kTokens at most one per lane
+  const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) - kConsumers;
+  const int my = quarter * kTokens + lane;  // this lane's token of a tile
   const int64_t first = place.run * blockIdx.x;
   const int count = static_cast<int>(min(place.run, place.total - first));
   int i = place.seq;
   Seq s = load_seq(p, i, false);
   SeqWork w = work_of<L>(p, s);
   int64_t begin = place.start;  // units before sequence i
-  int rt_tile = static_cast<int>(place.within % w.tiles);
+  int tile = static_cast<int>(place.within % w.tiles);
   int64_t rest = place.within / w.tiles;
   int rt = static_cast<int>(rest % w.row_tiles);
   int head = static_cast<int>(rest / w.row_tiles);
   Span v = span_of(p, s, 0, s.fresh);
 
-  // page ids of the lane's tokens, looked up one unit ahead
+  // the page id of the lane's token, looked up one unit ahead
   constexpr int kUnused = -0x7fffffff, kNoEntry = -0x7ffffffe;  // not a token of the tile; no such entry
-  int base, cnt, page[KT];
+  int base, cnt, page, ord;
   auto look_up = [&]() {
-    const bool in_head = rt_tile < w.head_tiles;
-    const int t = in_head ? rt_tile : rt_tile - w.head_tiles;
-    base = (in_head ? 0 : v.low) + t * kTile;
+    const bool in_head = tile < w.head_tiles;
+    base = (in_head ? 0 : v.low) + (in_head ? tile : tile - w.head_tiles) * kTile;
     cnt = min(kTile, (in_head ? v.head : v.end) - base);
-#pragma unroll
-    for (int k = 0; k < KT; ++k) {
-      const int t2 = lane + 32 * k;
-      page[k] = kUnused;
-      if (t2 < cnt) {
-        const int64_t e = static_cast<int64_t>(s.e0) + p.by_page.div(base + t2);
-        // (the id is not looked at here, so that the load stays in flight)
-        if (e >= 0 && e < p.indices_cap)
-          page[k] = __ldg(p.kv_indices + e);
-        else
-          page[k] = kNoEntry;
-      }
+    page = kUnused;
+    if (lane < kTokens && my < cnt) {
+      ord = p.by_page.div(base + my);
+      const int64_t e = static_cast<int64_t>(s.e0) + ord;
+      // (the id is not looked at here, so that the load stays in flight)
+      page = e >= 0 && e < p.indices_cap ? __ldg(p.kv_indices + e) : kNoEntry;
     }
   };
   look_up();
@@ -310,31 +305,37 @@ __device__ __forceinline__ void load_units(const AttnParams &p, const Place &pla
   for (int u = 0; u < count; ++u) {
     uint8_t *st = stages + stage * L::kStage;
     const uint32_t sk = smem_addr(st), sv = sk + L::kKV, sq = sv + L::kKV, ss = sq + L::kQ;
-    // this unit's numbers; the look-up of the next one overwrites them
-    const int tile = rt_tile, u_base = base, u_cnt = cnt, u_head = head, u_rt = rt;
-    const Seq us = s;
-    const SeqWork uw = w;
+    UnitInfo *info = reinterpret_cast<UnitInfo *>(st + L::kInfo);
+    const bool ok = page >= 0 && page < p.num_pages;
+    if (!ok && page != kUnused)
+      raise_deverr(p.error_word, page == kNoEntry ? YL_DEVERR_INDICES_CAP : YL_DEVERR_PAGE_RANGE);
+    const int64_t off = ok ? page * p.page_stride + (base + my - ord * p.page_size) * p.slot_stride + head * p.head_stride : 0;
+    const int64_t sc = ok ? page * p.scale_page_stride + head * p.scale_head_stride : 0;
+    const uint32_t valid = __ballot_sync(0xffffffffu, ok);
+    // this unit's description, before the state moves on
+    const bool is_first = u == 0 || tile == 0, ends = tile == w.tiles - 1;
+    const int rows = s.fresh * p.group, row0 = rt * kRows, pos0 = s.total - s.fresh, q0 = s.q0, u_base = base, u_head = head;
     const int64_t seg = begin + (static_cast<int64_t>(head) * w.row_tiles + rt) * w.tiles;  // its first unit in the line
-    int64_t off[KT], sc[KT];
-    uint32_t valid[KT];
-#pragma unroll
-    for (int k = 0; k < KT; ++k) {
-      const int t2 = lane + 32 * k;
-      const bool ok = page[k] >= 0 && page[k] < p.num_pages;
-      if (!ok && page[k] != kUnused)
-        raise_deverr(p.error_word, page[k] == kNoEntry ? YL_DEVERR_INDICES_CAP : YL_DEVERR_PAGE_RANGE);
-      const int pos = u_base + t2;
-      const int slot = pos - static_cast<int>(p.by_page.div(max(pos, 0))) * p.page_size;
-      off[k] = ok ? static_cast<int64_t>(page[k]) * p.page_stride + static_cast<int64_t>(slot) * p.slot_stride +
-                        u_head * p.head_stride
-                  : 0;
-      sc[k] = ok ? static_cast<int64_t>(page[k]) * p.scale_page_stride + u_head * p.scale_head_stride : 0;
-      valid[k] = __ballot_sync(0xffffffffu, ok);
+    int flags = is_first ? kFirst : 0;
+    if (ends || u == count - 1) flags |= kLast;
+    if (ends && seg >= first) flags |= kWhole;
+    const int last_pos = s.total - 1, end = base + cnt - 1;
+    const bool all = end <= pos0 && (p.window == 0 || base > last_pos - p.window || end < p.sinks);
+    if (s.fresh > 1 && !all) flags |= kRagged;
+    if (u == 0 && quarter == 0 && lane == 0) {
+      // where the parts of a result lie that began in an earlier CTA
+      int4 meta = make_int4(0, 0, 0, 0);
+      if (seg < first) {
+        const int c0 = static_cast<int>(seg / place.run), c1 = static_cast<int>((seg + w.tiles - 1) / place.run);
+        // the first CTA boundary inside it stands for the whole of it
+        if (c0 + 1 == static_cast<int>(blockIdx.x)) meta = make_int4(c1 - c0 + 1, q0, row0 | head << 16, rows);
+      }
+      p.meta[blockIdx.x] = meta;
     }
-    // on to the next unit's look-up, before this one's copies
+    // on to the next unit's look-up, in flight while this one is copied
     if (u + 1 < count) {
-      if (++rt_tile == w.tiles) {
-        rt_tile = 0;
+      if (++tile == w.tiles) {
+        tile = 0;
         if (++rt == w.row_tiles) {
           rt = 0;
           if (++head == p.heads) {
@@ -357,71 +358,47 @@ __device__ __forceinline__ void load_units(const AttnParams &p, const Place &pla
     constexpr int kRowsPer = 32 / L::kChunks;  // rows of one copy instruction
     const int c = lane % L::kChunks;
 #pragma unroll
-    for (int j = 0; j < kTile / kRowsPer; ++j) {
+    for (int j = 0; j < kTokens / kRowsPer; ++j) {
       const int r = j * kRowsPer + lane / L::kChunks;
-      const int k = j * kRowsPer / 32;
-      const int64_t o = __shfl_sync(0xffffffffu, off[k], r & 31) + c * 16;
-      const bool ok = (valid[k] >> (r & 31)) & 1u;
-      const int at = chunk_at<D, Q8>(r, c);
-      cp_async16(sk + at, p.kv[0] + o, ok);
-      cp_async16(sv + at, p.kv[1] + o, ok);
+      const int64_t o = __shfl_sync(0xffffffffu, off, r) + c * 16;
+      const bool good = (valid >> r) & 1u;
+      const int at = chunk_at<D, Q8>(quarter * kTokens + r, c);
+      cp_async16(sk + at, p.kv[0] + o, good);
+      cp_async16(sv + at, p.kv[1] + o, good);
     }
-    if (Q8) {
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        const bool ok = (valid[k] >> lane) & 1u;
-        cp_async4(ss + (lane + 32 * k) * 4, p.scale[0] + sc[k], ok);
-        cp_async4(ss + kTile * 4 + (lane + 32 * k) * 4, p.scale[1] + sc[k], ok);
-      }
+    if (Q8 && lane < kTokens) {
+      cp_async4(ss + my * 4, p.scale[0] + sc, ok);
+      cp_async4(ss + (kTile + my) * 4, p.scale[1] + sc, ok);
     }
-    const bool is_first = u == 0 || tile == 0;
-    const int rows = us.fresh * p.group;
     if (is_first) {
       constexpr int kQChunks = D / 8;
 #pragma unroll
-      for (int j = 0; j < kRows * kQChunks / 32; ++j) {
-        const int n = j * 32 + lane, r = n / kQChunks, qc = n % kQChunks;
-        const int row = u_rt * kRows + r;
+      for (int j = 0; j < (kRows * kQChunks + 127) / 128; ++j) {
+        const int n = (j * kConsumers + quarter) * 32 + lane, r = n / kQChunks, qc = n % kQChunks;
+        if (n >= kRows * kQChunks) break;
+        const int row = row0 + r;
         const int t = p.by_group.div(row), g = row - t * p.group;
-        const int64_t qrow = static_cast<int64_t>(us.q0) + t;
-        const bool ok = row < rows && qrow < p.num_tokens;
-        const char *src = p.q + (ok ? qrow * p.q_row_stride + (static_cast<int64_t>(u_head) * p.group + g) * p.q_head_stride
-                                    : 0) + qc * 16;
-        cp_async16(sq + r * D * 2 + (((qc & ~7) | ((qc ^ r) & 7)) << 4), src, ok);
+        const int64_t qrow = static_cast<int64_t>(q0) + t;
+        const bool has = row < rows && qrow < p.num_tokens;
+        const char *src =
+            p.q + (has ? qrow * p.q_row_stride + (static_cast<int64_t>(u_head) * p.group + g) * p.q_head_stride : 0) + qc * 16;
+        cp_async16(sq + r * D * 2 + (((qc & ~7) | ((qc ^ r) & 7)) << 4), src, has);
       }
     }
     cp_async_arrive(smem_addr(full + stage));
     if (lane == 0) {
-      UnitInfo info;
-#pragma unroll
-      for (int k = 0; k < KT; ++k) info.valid[k] = valid[k];
-      info.base = u_base;
-      info.pos0 = us.total - us.fresh;
-      info.row0 = u_rt * kRows;
-      info.rows = rows;
-      info.q0 = us.q0;
-      info.head = u_head;
-      int flags = is_first ? kFirst : 0;
-      const bool ends = tile == uw.tiles - 1;
-      if (ends || u == count - 1) flags |= kLast;
-      if (ends && seg >= first) flags |= kWhole;
-      const int last_pos = us.total - 1, end = u_base + u_cnt - 1;
-      const bool all = end <= info.pos0 && (p.window == 0 || u_base > last_pos - p.window || end < p.sinks);
-      if (us.fresh > 1 && !all) flags |= kRagged;
-      info.flags = flags;
-      info.part = static_cast<int>(2 * blockIdx.x + (seg >= first ? 1 : 0));
-      *reinterpret_cast<UnitInfo *>(st + L::kInfo) = info;
-      mbar_arrive(full + stage);
-      // where the parts of a result lie that began in an earlier CTA
-      if (u == 0) {
-        int4 meta = make_int4(0, 0, 0, 0);
-        if (seg < first) {
-          const int c0 = static_cast<int>(seg / place.run), c1 = static_cast<int>((seg + uw.tiles - 1) / place.run);
-          // the first CTA boundary inside it stands for the whole of it
-          if (c0 + 1 == static_cast<int>(blockIdx.x)) meta = make_int4(c1 - c0 + 1, us.q0, info.row0 | u_head << 16, rows);
-        }
-        p.meta[blockIdx.x] = meta;
+      info->valid[quarter] = valid;
+      if (quarter == 0) {
+        info->base = u_base;
+        info->pos0 = pos0;
+        info->row0 = row0;
+        info->rows = rows;
+        info->q0 = q0;
+        info->head = u_head;
+        info->flags = flags;
+        info->part = static_cast<int>(2 * blockIdx.x + (seg >= first ? 1 : 0));
       }
+      mbar_arrive(full + stage);
     }
     if (++stage == L::kStages) {
       stage = 0;
@@ -552,7 +529,7 @@ __device__ __forceinline__ void compute_units(const AttnParams &p, const Place &
         }
     }
     // bit i: token t0 + i of the tile
-    const uint32_t valid = (info->valid[t0 >> 5] >> (t0 & 31)) & (L::kTokens == 32 ? 0xffffffffu : 0xffffu);
+    const uint32_t valid = info->valid[warp];
     float vs[MT][2], vtop = vref;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -833,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, Q8, NB>::kCtas)
   uint64_t *empty = full + L::kStages, *joined = empty + L::kStages;
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kStages; ++i) {
-      mbar_init(full + i, 33);  // the loading warp's copies, and its descriptor
+      mbar_init(full + i, kConsumers * 33);  // the loading warps' copies, and their descriptions
       mbar_init(empty + i, kConsumers);
     }
     mbar_init(joined, kConsumers);
@@ -847,10 +824,14 @@ __global__ void __launch_bounds__(kThreads, Layout<D, Q8, NB>::kCtas)
     if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
-  if (threadIdx.x >= kConsumers * 32)
+  if (threadIdx.x >= kConsumers * 32) {
+    if (L::kCtas == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     load_units<D, Q8, NB>(p, place, stages, full, empty);
-  else
+  } else {
+    // two CTAs: their 2 x 256 x 128 registers, 176 for a computing thread
+    if (L::kCtas == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     compute_units<T, D, Q8, NB>(p, place, stages, full, empty, joined, merge);
+  }
 }
 
 // Joins the parts of a result that began in CTA c - 1 and goes on in CTA c (and
