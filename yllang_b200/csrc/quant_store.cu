@@ -65,15 +65,31 @@ __device__ __forceinline__ Touched find_page(const QuantStoreParams &p, uint32_t
   r.page = r.row0 = 0;
   r.held = 0;
   const int ps = p.pool.page_size;
-  const int i = warp_find(p.batch, cand, lane, [&](int s) -> int64_t {
-    const int64_t q = __ldg(p.qo_indptr + s);
-    return BY_TOKEN ? q : q / ps + 2ll * s;
-  });
-  const int64_t q0 = __ldg(p.qo_indptr + i), q1 = __ldg(p.qo_indptr + i + 1);
-  const int64_t e0 = __ldg(p.kv_indptr + i), e1 = __ldg(p.kv_indptr + i + 1);
+  int i = 0;
+  int64_t q0, q1, e0, e1;
+  int last;
+  auto load = [&]() {
+    q0 = __ldg(p.qo_indptr + i);
+    q1 = __ldg(p.qo_indptr + i + 1);
+    e0 = __ldg(p.kv_indptr + i);
+    e1 = __ldg(p.kv_indptr + i + 1);
+    last = __ldg(p.last_len + i);
+  };
+  if (BY_TOKEN) {
+    // in a decode batch row n is sequence n's, which saves the search's loads
+    i = static_cast<int>(min(cand, static_cast<uint32_t>(p.batch - 1)));
+    load();
+  }
+  if (!BY_TOKEN || q0 > cand || q1 <= cand) {
+    i = warp_find(p.batch, cand, lane, [&](int s) -> int64_t {
+      const int64_t q = __ldg(p.qo_indptr + s);
+      return BY_TOKEN ? q : q / ps + 2ll * s;
+    });
+    load();
+  }
   const int64_t fresh = q1 - q0, pages = e1 - e0;
   if (fresh <= 0 || q0 < 0) return r;
-  const int last = min(max(__ldg(p.last_len + i), 0), ps);
+  last = min(max(last, 0), ps);
   const int64_t total = pages > 0 ? (pages - 1) * ps + last : 0;
   const int64_t prior = total - fresh;
   int64_t ord;
@@ -163,32 +179,33 @@ __device__ __forceinline__ void requantise(uint8_t *codes, int64_t slot_stride, 
   }
 }
 
-// PB planes of one page at once, each with at most RB new tokens held in
-// registers (STREAM: any number, read twice).
+// This lane's part of the first row of a page's new tokens in a plane.
+template <int D>
+__device__ __forceinline__ const char *row_of(const QuantStoreParams &p, int64_t row0, int plane, int h, int lane) {
+  const int kv = plane & 1, layer = plane >> 1;
+  return p.x[kv] + layer * p.layer_stride[kv] + row0 * p.row_stride[kv] + static_cast<int64_t>(h) * (D * 2) +
+         lane % (D / 8) * 16;
+}
+
+// PB planes of one page at once, each with at most RB new tokens, which x holds
+// (STREAM: any number, read twice).
 template <typename T, int D, int PB, int RB, bool STREAM>
 __device__ __forceinline__ void store_planes(const QuantStoreParams &p, const Touched &pg, int plane0, int count,
-                                             int head, int lane) {
+                                             int head, int lane, uint4 (&x)[PB][RB]) {
   constexpr int LPR = D / 8;
   const int sub = lane % LPR;
   const bool active = head < p.pool.num_heads;
   const int h = active ? head : 0;
-  uint4 x[PB][RB];
   float old[PB];
   const char *src[PB];
 #pragma unroll
   for (int b = 0; b < PB; ++b) {
     const int plane = plane0 + b, kv = plane & 1, layer = plane >> 1;
-    src[b] = p.x[kv] + layer * p.layer_stride[kv] + pg.row0 * p.row_stride[kv] + static_cast<int64_t>(h) * (D * 2) +
-             sub * 16;
+    src[b] = row_of<D>(p, pg.row0, plane, h, lane);
     old[b] = 0.f;
-    if (b < count && active) {
-#pragma unroll
-      for (int r = 0; r < RB; ++r)
-        if (!STREAM && r < pg.count) x[b][r] = __ldg(reinterpret_cast<const uint4 *>(src[b] + r * p.row_stride[kv]));
-      if (pg.held > 0)
-        old[b] = p.pool.scale[kv][layer * p.pool.scale_layer_stride + pg.page * p.pool.scale_page_stride +
-                                  h * p.pool.scale_head_stride];
-    }
+    if (b < count && active && pg.held > 0)
+      old[b] = p.pool.scale[kv][layer * p.pool.scale_layer_stride + pg.page * p.pool.scale_page_stride +
+                                h * p.pool.scale_head_stride];
   }
 #pragma unroll
   for (int b = 0; b < PB; ++b) {
@@ -268,26 +285,62 @@ __device__ __forceinline__ void store_planes(const QuantStoreParams &p, const To
   }
 }
 
+// By token (batches of mostly one new token a sequence): a warp's first rows are
+// known before its page is, so they are loaded in front of the look-ups; eight
+// planes at once.  By page: up to 16 rows of a page at once.  Two kernels, since
+// the second's registers would halve the warps that hide the first's latency.
 template <typename T, int D, bool BY_TOKEN>
-__global__ void __launch_bounds__(kStoreThreads) quant_store_kernel(const __grid_constant__ QuantStoreParams p) {
+__global__ void __launch_bounds__(kStoreThreads, BY_TOKEN ? 7 : 4)
+    quant_store_kernel(const __grid_constant__ QuantStoreParams p) {
   constexpr int RPW = 32 / (D / 8);  // heads a warp takes at once
+  constexpr int PB = 8;              // planes at once, by token
   const int lane = threadIdx.x & 31;
   const uint32_t unit = blockIdx.x * (kStoreThreads / 32) + (threadIdx.x >> 5);
   pdl_wait();  // rows and page arrays may be written by the kernel just before this one
   const uint32_t chunk = unit % p.chunks, rest = unit / p.chunks;
   const uint32_t cand = rest % p.cands, run = rest / p.cands;
   if (run >= p.runs) return;
-  const Touched pg = find_page<BY_TOKEN>(p, cand, lane, chunk == 0 && run == 0 && lane == 0);
-  if (pg.count == 0) return;
   const int head = static_cast<int>(chunk) * RPW + lane / (D / 8);
+  const bool active = head < p.pool.num_heads;
+  const int h = active ? head : 0;
   const int first = run * p.planes_per_run;
   const int end = min(first + static_cast<int>(p.planes_per_run), p.planes);
-  if (pg.count == 1) {
-    for (int pl = first; pl < end; pl += 8) store_planes<T, D, 8, 1, false>(p, pg, pl, end - pl, head, lane);
-  } else if (pg.count <= 16) {
-    for (int pl = first; pl < end; ++pl) store_planes<T, D, 1, 16, false>(p, pg, pl, 1, head, lane);
+  const bool report = chunk == 0 && run == 0 && lane == 0;
+  if (BY_TOKEN) {
+    uint4 x[PB][1];
+    auto load = [&](int plane0) {
+#pragma unroll
+      for (int b = 0; b < PB; ++b)
+        if (plane0 + b < end && active) x[b][0] = __ldg(reinterpret_cast<const uint4 *>(row_of<D>(p, cand, plane0 + b, h, lane)));
+    };
+    load(first);
+    const Touched pg = find_page<BY_TOKEN>(p, cand, lane, report);
+    if (pg.count == 0) return;
+    if (pg.count == 1 && pg.row0 == cand) {
+      for (int pl = first; pl < end; pl += PB) {
+        if (pl > first) load(pl);
+        store_planes<T, D, PB, 1, false>(p, pg, pl, end - pl, head, lane, x);
+      }
+    } else {
+      uint4 none[1][1];
+      for (int pl = first; pl < end; ++pl) store_planes<T, D, 1, 1, true>(p, pg, pl, 1, head, lane, none);
+    }
   } else {
-    for (int pl = first; pl < end; ++pl) store_planes<T, D, 1, 1, true>(p, pg, pl, 1, head, lane);
+    const Touched pg = find_page<BY_TOKEN>(p, cand, lane, report);
+    if (pg.count == 0) return;
+    if (pg.count <= 16) {
+      for (int pl = first; pl < end; ++pl) {
+        uint4 x[1][16];
+        const char *src = row_of<D>(p, pg.row0, pl, h, lane);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (r < pg.count && active) x[0][r] = __ldg(reinterpret_cast<const uint4 *>(src + r * p.row_stride[pl & 1]));
+        store_planes<T, D, 1, 16, false>(p, pg, pl, 1, head, lane, x);
+      }
+    } else {
+      uint4 none[1][1];
+      for (int pl = first; pl < end; ++pl) store_planes<T, D, 1, 1, true>(p, pg, pl, 1, head, lane, none);
+    }
   }
 }
 
@@ -310,7 +363,7 @@ struct QuantLoadParams {
 constexpr int kLoadThreads = 256;
 constexpr int kLoadRows = 4;
 
-template <typename T, int D, typename Slot>
+template <typename T, int D, typename Slot, bool WIDE>
 __global__ void __launch_bounds__(kLoadThreads) quant_load_kernel(const __grid_constant__ QuantLoadParams p) {
   constexpr int LPR = D / 16;
   constexpr int GROUPS = kLoadThreads / LPR;
@@ -365,8 +418,14 @@ __global__ void __launch_bounds__(kLoadThreads) quant_load_kernel(const __grid_c
         b = b > T::kMax ? T::kMax : b < -T::kMax ? -T::kMax : b;
         o[i] = T::pack(a, b);
       }
-      reinterpret_cast<uint4 *>(dst[u])[0] = make_uint4(o[0], o[1], o[2], o[3]);
-      reinterpret_cast<uint4 *>(dst[u])[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      if (WIDE) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst[u]), "r"(o[0]), "r"(o[1]), "r"(o[2]),
+                     "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
+                     : "memory");
+      } else {
+        reinterpret_cast<uint4 *>(dst[u])[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        reinterpret_cast<uint4 *>(dst[u])[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      }
     }
   }
 }
@@ -485,10 +544,12 @@ extern "C" int yl_kv_quant_store(const yl_quant_store_args *a, cudaStream_t stre
   p.cands = static_cast<uint32_t>(by_token ? a->num_tokens : by_page);
   const int heads_per_warp = 256 / a->pool.head_dim;
   p.chunks = static_cast<uint32_t>((a->pool.num_heads + heads_per_warp - 1) / heads_per_warp);
-  // enough units for two waves of resident warps, a run of planes each
+  // By token a wave of resident warps, a run of planes each; by page, where a
+  // warp's work is longer, up to four waves.
   const uint64_t items = static_cast<uint64_t>(p.cands) * p.chunks;
-  const uint64_t want = static_cast<uint64_t>(sm_count()) * 64;
-  const uint64_t runs = std::min<uint64_t>(std::max<uint64_t>((want + items - 1) / items, 1), p.planes);
+  const uint64_t want = static_cast<uint64_t>(sm_count()) * (by_token ? 28 : 64);
+  const uint64_t runs =
+      std::min<uint64_t>(std::max<uint64_t>(by_token ? want / items : (want + items - 1) / items, 1), p.planes);
   p.planes_per_run = static_cast<uint32_t>((p.planes + runs - 1) / runs);
   p.runs = (p.planes + p.planes_per_run - 1) / p.planes_per_run;
   const uint64_t units = items * p.runs;
@@ -545,7 +606,12 @@ extern "C" int yl_kv_quant_load(const yl_quant_load_args *a, cudaStream_t stream
   return pick_type_dim(a->dtype, a->pool.head_dim, [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
-    auto fn = a->slot_is_int64 ? quant_load_kernel<T, D, int64_t> : quant_load_kernel<T, D, int32_t>;
+    // 32-byte stores where rows and strides allow them
+    const bool wide = ((reinterpret_cast<uintptr_t>(a->k_out) | reinterpret_cast<uintptr_t>(a->v_out) |
+                        static_cast<uintptr_t>(p.row_stride[0] | p.row_stride[1] | p.layer_stride[0] | p.layer_stride[1])) &
+                       31u) == 0;
+    auto fn = a->slot_is_int64 ? (wide ? quant_load_kernel<T, D, int64_t, true> : quant_load_kernel<T, D, int64_t, false>)
+                               : (wide ? quant_load_kernel<T, D, int32_t, true> : quant_load_kernel<T, D, int32_t, false>);
     const uint64_t per_block = static_cast<uint64_t>(kLoadThreads / (D / 16)) * kLoadRows;
     const uint64_t want = (p.rows + per_block - 1) / per_block;
     const uint64_t cap = static_cast<uint64_t>(sm_count()) * 8;
