@@ -162,8 +162,8 @@ __device__ __forceinline__ uint2 quantise8(const uint4 &w, float inv) {
 }
 
 // Held tokens take the page's new scale (each code times old / new, rounded).
-__device__ __forceinline__ void requantise(uint8_t *codes, int64_t slot_stride, int held, float ratio) {
-  for (int t = 0; t < held; ++t) {
+__device__ __forceinline__ void requantise(uint8_t *codes, int64_t slot_stride, int first, int held, int step, float ratio) {
+  for (int t = first; t < held; t += step) {
     uint2 *at = reinterpret_cast<uint2 *>(codes + t * slot_stride);
     const uint2 w = *at;
     const uint32_t v[2] = {w.x, w.y};
@@ -179,6 +179,27 @@ __device__ __forceinline__ void requantise(uint8_t *codes, int64_t slot_stride, 
   }
 }
 
+// The page's scale for new tokens with this largest element, and whether it is
+// to be written; ratio != 1: held codes are to be multiplied by it.
+struct NewScale {
+  float scale, ratio;
+  bool write;
+};
+__device__ __forceinline__ NewScale new_scale(const QuantStoreParams &p, float amax, int held, float old, bool report) {
+  NewScale n{scale_for(amax), 1.f, true};
+  if (held > 0) {
+    if (!good_scale(old)) {
+      if (report) raise_deverr(p.error_word, YL_DEVERR_SCALE);
+    } else if (n.scale > old) {
+      n.ratio = old / n.scale;
+    } else {
+      n.scale = old;
+      n.write = false;
+    }
+  }
+  return n;
+}
+
 // This lane's part of the first row of a page's new tokens in a plane.
 template <int D>
 __device__ __forceinline__ const char *row_of(const QuantStoreParams &p, int64_t row0, int plane, int h, int lane) {
@@ -187,9 +208,8 @@ __device__ __forceinline__ const char *row_of(const QuantStoreParams &p, int64_t
          lane % (D / 8) * 16;
 }
 
-// PB planes of one page at once, each with at most RB new tokens, which x holds
-// (STREAM: any number, read twice).
-template <typename T, int D, int PB, int RB, bool STREAM>
+// PB planes of one page at once, each with at most RB new tokens, which x holds.
+template <typename T, int D, int PB, int RB>
 __device__ __forceinline__ void store_planes(const QuantStoreParams &p, const Touched &pg, int plane0, int count,
                                              int head, int lane, uint4 (&x)[PB][RB]) {
   constexpr int LPR = D / 8;
@@ -213,22 +233,9 @@ __device__ __forceinline__ void store_planes(const QuantStoreParams &p, const To
     const int64_t stride = p.row_stride[kv];
     uint32_t m = 0;
     if (b < count && active) {
-      if (STREAM) {
-        for (int r = 0; r < pg.count; r += 8) {
-          uint4 w[8];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            w[u] = make_uint4(0, 0, 0, 0);
-            if (r + u < pg.count) w[u] = __ldg(reinterpret_cast<const uint4 *>(src[b] + (r + u) * stride));
-          }
-#pragma unroll
-          for (int u = 0; u < 8; ++u) m = abs_max8(m, w[u]);
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < RB; ++r)
-          if (r < pg.count) m = abs_max8(m, x[b][r]);
-      }
+      for (int r = 0; r < RB; ++r)
+        if (r < pg.count) m = abs_max8(m, x[b][r]);
     }
 #pragma unroll
     for (int d = LPR / 2; d > 0; d >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
@@ -250,96 +257,189 @@ __device__ __forceinline__ void store_planes(const QuantStoreParams &p, const To
                      h * p.pool.head_stride + sub * 8;
       float *sc = p.pool.scale[kv] + layer * p.pool.scale_layer_stride + pg.page * p.pool.scale_page_stride +
                   h * p.pool.scale_head_stride;
-      float scale = scale_for(amax);
-      bool write = true;
-      if (pg.held > 0) {
-        if (!good_scale(old[b])) {
-          if (sub == 0) raise_deverr(p.error_word, YL_DEVERR_SCALE);
-        } else if (scale > old[b]) {
-          requantise(dst, p.pool.slot_stride, pg.held, old[b] / scale);
-        } else {
-          scale = old[b];
-          write = false;
-        }
-      }
-      if (write && sub == 0) *sc = scale;
-      const float inv = 1.f / scale;  // exact for a power of two
+      const NewScale n = new_scale(p, amax, pg.held, old[b], sub == 0);
+      if (n.ratio != 1.f) requantise(dst, p.pool.slot_stride, 0, pg.held, 1, n.ratio);
+      if (n.write && sub == 0) *sc = n.scale;
+      const float inv = 1.f / n.scale;  // exact for a power of two
       dst += pg.held * p.pool.slot_stride;
-      if (STREAM) {
-        for (int r = 0; r < pg.count; r += 8) {
-          uint4 w[8];
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            if (r + u < pg.count) w[u] = __ldg(reinterpret_cast<const uint4 *>(src[b] + (r + u) * stride));
+      for (int r = 0; r < RB; ++r)
+        if (r < pg.count) *reinterpret_cast<uint2 *>(dst + r * p.pool.slot_stride) = quantise8<T>(x[b][r], inv);
+    }
+  }
+}
+
+// A page of several new tokens in a batch of mostly one each: rows read twice.
+template <typename T, int D>
+__device__ __noinline__ void store_rows_twice(const QuantStoreParams &p, const Touched &pg, int plane, int head, int lane) {
+  constexpr int LPR = D / 8;
+  const int kv = plane & 1, layer = plane >> 1, sub = lane % LPR;
+  const bool active = head < p.pool.num_heads;
+  const int h = active ? head : 0;
+  const int64_t stride = p.row_stride[kv];
+  const char *src = row_of<D>(p, pg.row0, plane, h, lane);
+  float amax = 0.f;
+  bool bad = false;
+  if (active)
+    for (int r = 0; r < pg.count; ++r) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4 *>(src + r * stride));
+      const uint32_t m = abs_max8(0, w);
+      bad |= max(m & 0xffffu, m >> 16) >= T::kInf;
+      amax = finite_abs_max8<T>(amax, w);
+    }
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            if (r + u < pg.count)
-              *reinterpret_cast<uint2 *>(dst + (r + u) * p.pool.slot_stride) = quantise8<T>(w[u], inv);
-        }
-      } else {
+  for (int d = LPR / 2; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+  if (bad) raise_deverr(p.error_word, YL_DEVERR_NONFINITE);
+  if (!active) return;
+  uint8_t *dst = p.pool.codes[kv] + layer * p.pool.layer_stride + pg.page * p.pool.page_stride + h * p.pool.head_stride +
+                 sub * 8;
+  float *sc = p.pool.scale[kv] + layer * p.pool.scale_layer_stride + pg.page * p.pool.scale_page_stride +
+              h * p.pool.scale_head_stride;
+  const float old = pg.held > 0 ? *sc : 0.f;
+  const NewScale n = new_scale(p, amax, pg.held, old, sub == 0);
+  if (n.ratio != 1.f) requantise(dst, p.pool.slot_stride, 0, pg.held, 1, n.ratio);
+  __syncwarp(__activemask());  // every lane has the old scale
+  if (n.write && sub == 0) *sc = n.scale;
+  const float inv = 1.f / n.scale;  // exact for a power of two
+  dst += pg.held * p.pool.slot_stride;
+  for (int r = 0; r < pg.count; ++r)
+    *reinterpret_cast<uint2 *>(dst + r * p.pool.slot_stride) =
+        quantise8<T>(__ldg(reinterpret_cast<const uint4 *>(src + r * stride)), inv);
+}
+
+// How a page's new tokens are dealt out.  kByToken (batches of mostly one new
+// token a sequence, and pages of one): a warp's first rows are known before its
+// page is, so they are loaded in front of the look-ups, eight planes at once.
+// kByWarp: up to 16 rows of a page by a warp.  kByBlock (pages of more than 16
+// tokens): four warps share a page, up to 64 rows in registers, and exchange
+// their maxima; of longer pages the rows are read twice.  They are kernels of
+// their own, since the registers of one would cost the other's warps in flight.
+enum StoreMode { kByToken, kByWarp, kByBlock };
+
+template <typename T, int D>
+__device__ __forceinline__ void store_by_block(const QuantStoreParams &p, const Touched &pg, int first, int end, int head,
+                                               int lane) {
+  constexpr int LPR = D / 8, RPW = 32 / LPR, TEAM = kStoreThreads / 32, SLAB = 16 * TEAM;
+  __shared__ uint32_t bits[2][TEAM][RPW];
+  __shared__ float finite[TEAM][RPW];
+  const int warp = threadIdx.x >> 5, sub = lane % LPR, group = lane / LPR;
+  const bool active = head < p.pool.num_heads;
+  const int h = active ? head : 0;
+  for (int pl = first; pl < end; ++pl) {
+    const int kv = pl & 1, layer = pl >> 1, par = pl & 1;
+    const int64_t stride = p.row_stride[kv];
+    const char *src = row_of<D>(p, pg.row0, pl, h, lane);
+    float *sc = p.pool.scale[kv] + layer * p.pool.scale_layer_stride + pg.page * p.pool.scale_page_stride +
+                h * p.pool.scale_head_stride;
+    const float old = active && pg.held > 0 ? *sc : 0.f;
+    uint4 x[16];
+    auto load = [&](int slab) {
 #pragma unroll
-        for (int r = 0; r < RB; ++r)
-          if (r < pg.count) *reinterpret_cast<uint2 *>(dst + r * p.pool.slot_stride) = quantise8<T>(x[b][r], inv);
+      for (int r = 0; r < 16; ++r) {
+        const int row = slab + r * TEAM + warp;
+        x[r] = make_uint4(0, 0, 0, 0);
+        if (row < pg.count && active) x[r] = __ldg(reinterpret_cast<const uint4 *>(src + row * stride));
+      }
+    };
+    uint32_t m = 0;
+    for (int slab = 0; slab < pg.count; slab += SLAB) {
+      load(slab);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = abs_max8(m, x[r]);
+    }
+#pragma unroll
+    for (int d = LPR / 2; d > 0; d >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if (sub == 0) bits[par][warp][group] = max(m & 0xffffu, m >> 16);
+    // (the barrier also ends the reading of a held scale, which is written below,
+    // and of bits two planes back)
+    __syncthreads();
+    m = bits[par][0][group];
+#pragma unroll
+    for (int w = 1; w < TEAM; ++w) m = max(m, bits[par][w][group]);
+    float amax = T::unpack(m).x;
+    if (__syncthreads_or(m >= T::kInf)) {  // an infinity or NaN: the finite maximum, the slow way
+      float f = 0.f;
+      if (active)
+        for (int row = warp; row < pg.count; row += TEAM)
+          f = finite_abs_max8<T>(f, __ldg(reinterpret_cast<const uint4 *>(src + row * stride)));
+#pragma unroll
+      for (int d = LPR / 2; d > 0; d >>= 1) f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, d));
+      if (sub == 0) finite[warp][group] = f;
+      __syncthreads();
+      amax = finite[0][group];
+#pragma unroll
+      for (int w = 1; w < TEAM; ++w) amax = fmaxf(amax, finite[w][group]);
+      __syncthreads();
+      if (m >= T::kInf && sub == 0 && warp == 0) raise_deverr(p.error_word, YL_DEVERR_NONFINITE);
+    }
+    if (!active) continue;
+    uint8_t *dst = p.pool.codes[kv] + layer * p.pool.layer_stride + pg.page * p.pool.page_stride + h * p.pool.head_stride +
+                   sub * 8;
+    const NewScale n = new_scale(p, amax, pg.held, old, sub == 0 && warp == 0);
+    if (n.ratio != 1.f) requantise(dst, p.pool.slot_stride, warp, pg.held, TEAM, n.ratio);
+    if (n.write && sub == 0 && warp == 0) *sc = n.scale;
+    const float inv = 1.f / n.scale;  // exact for a power of two
+    dst += pg.held * p.pool.slot_stride;
+    for (int slab = 0; slab < pg.count; slab += SLAB) {
+      if (pg.count > SLAB) load(slab);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = slab + r * TEAM + warp;
+        if (row < pg.count) *reinterpret_cast<uint2 *>(dst + row * p.pool.slot_stride) = quantise8<T>(x[r], inv);
       }
     }
   }
 }
 
-// By token (batches of mostly one new token a sequence): a warp's first rows are
-// known before its page is, so they are loaded in front of the look-ups; eight
-// planes at once.  By page: up to 16 rows of a page at once.  Two kernels, since
-// the second's registers would halve the warps that hide the first's latency.
-template <typename T, int D, bool BY_TOKEN>
-__global__ void __launch_bounds__(kStoreThreads, BY_TOKEN ? 7 : 4)
+template <typename T, int D, StoreMode MODE>
+__global__ void __launch_bounds__(kStoreThreads, MODE == kByToken ? 7 : 4)
     quant_store_kernel(const __grid_constant__ QuantStoreParams p) {
   constexpr int RPW = 32 / (D / 8);  // heads a warp takes at once
   constexpr int PB = 8;              // planes at once, by token
   const int lane = threadIdx.x & 31;
-  const uint32_t unit = blockIdx.x * (kStoreThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t unit = MODE == kByBlock ? blockIdx.x : blockIdx.x * (kStoreThreads / 32) + (threadIdx.x >> 5);
   pdl_wait();  // rows and page arrays may be written by the kernel just before this one
-  const uint32_t chunk = unit % p.chunks, rest = unit / p.chunks;
+  const uint32_t part = unit % p.chunks, rest = unit / p.chunks;
   const uint32_t cand = rest % p.cands, run = rest / p.cands;
   if (run >= p.runs) return;
-  const int head = static_cast<int>(chunk) * RPW + lane / (D / 8);
-  const bool active = head < p.pool.num_heads;
-  const int h = active ? head : 0;
   const int first = run * p.planes_per_run;
   const int end = min(first + static_cast<int>(p.planes_per_run), p.planes);
-  const bool report = chunk == 0 && run == 0 && lane == 0;
-  if (BY_TOKEN) {
+  const bool report = part == 0 && run == 0 && lane == 0 && (MODE != kByBlock || threadIdx.x == 0);
+  const int head = static_cast<int>(part) * RPW + lane / (D / 8);
+  if (MODE == kByToken) {
     uint4 x[PB][1];
     auto load = [&](int plane0) {
 #pragma unroll
       for (int b = 0; b < PB; ++b)
-        if (plane0 + b < end && active) x[b][0] = __ldg(reinterpret_cast<const uint4 *>(row_of<D>(p, cand, plane0 + b, h, lane)));
+        if (plane0 + b < end && head < p.pool.num_heads)
+          x[b][0] = __ldg(reinterpret_cast<const uint4 *>(row_of<D>(p, cand, plane0 + b, head, lane)));
     };
     load(first);
-    const Touched pg = find_page<BY_TOKEN>(p, cand, lane, report);
+    const Touched pg = find_page<true>(p, cand, lane, report);
     if (pg.count == 0) return;
-    if (pg.count == 1 && pg.row0 == cand) {
+    if (pg.count == 1) {  // then it is row `cand`
       for (int pl = first; pl < end; pl += PB) {
         if (pl > first) load(pl);
-        store_planes<T, D, PB, 1, false>(p, pg, pl, end - pl, head, lane, x);
+        store_planes<T, D, PB, 1>(p, pg, pl, end - pl, head, lane, x);
       }
     } else {
-      uint4 none[1][1];
-      for (int pl = first; pl < end; ++pl) store_planes<T, D, 1, 1, true>(p, pg, pl, 1, head, lane, none);
+      for (int pl = first; pl < end; ++pl) store_rows_twice<T, D>(p, pg, pl, head, lane);
     }
   } else {
-    const Touched pg = find_page<BY_TOKEN>(p, cand, lane, report);
+    const Touched pg = find_page<false>(p, cand, lane, report);
     if (pg.count == 0) return;
-    if (pg.count <= 16) {
+    if (MODE == kByBlock) {
+      store_by_block<T, D>(p, pg, first, end, head, lane);
+    } else {
       for (int pl = first; pl < end; ++pl) {
         uint4 x[1][16];
-        const char *src = row_of<D>(p, pg.row0, pl, h, lane);
+        const bool active = head < p.pool.num_heads;
+        const char *src = row_of<D>(p, pg.row0, pl, active ? head : 0, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (r < pg.count && active) x[0][r] = __ldg(reinterpret_cast<const uint4 *>(src + r * p.row_stride[pl & 1]));
-        store_planes<T, D, 1, 16, false>(p, pg, pl, 1, head, lane, x);
+        store_planes<T, D, 1, 16>(p, pg, pl, 1, head, lane, x);
       }
-    } else {
-      uint4 none[1][1];
-      for (int pl = first; pl < end; ++pl) store_planes<T, D, 1, 1, true>(p, pg, pl, 1, head, lane, none);
     }
   }
 }
@@ -542,24 +642,28 @@ extern "C" int yl_kv_quant_store(const yl_quant_store_args *a, cudaStream_t stre
   const int64_t by_page = a->num_tokens / a->pool.page_size + 2ll * a->batch_size;
   const bool by_token = a->num_tokens <= by_page;
   p.cands = static_cast<uint32_t>(by_token ? a->num_tokens : by_page);
+  const StoreMode mode = by_token ? kByToken : a->pool.page_size <= 16 ? kByWarp : kByBlock;
   const int heads_per_warp = 256 / a->pool.head_dim;
   p.chunks = static_cast<uint32_t>((a->pool.num_heads + heads_per_warp - 1) / heads_per_warp);
-  // By token a wave of resident warps, a run of planes each; by page, where a
-  // warp's work is longer, up to four waves.
-  const uint64_t items = static_cast<uint64_t>(p.cands) * p.chunks;
-  const uint64_t want = static_cast<uint64_t>(sm_count()) * (by_token ? 28 : 64);
-  const uint64_t runs =
-      std::min<uint64_t>(std::max<uint64_t>(by_token ? want / items : (want + items - 1) / items, 1), p.planes);
+  const uint64_t resident = static_cast<uint64_t>(sm_count()) * (mode == kByToken ? 28 : 16);  // warps
+  // By token a wave of resident warps; by page, where a warp's work is longer, up
+  // to four waves.
+  const uint64_t items = static_cast<uint64_t>(p.cands) * p.chunks * (mode == kByBlock ? 4 : 1);
+  const uint64_t runs = std::min<uint64_t>(
+      std::max<uint64_t>(mode == kByToken ? resident / items : (4 * resident + items - 1) / items, 1), p.planes);
   p.planes_per_run = static_cast<uint32_t>((p.planes + runs - 1) / runs);
   p.runs = (p.planes + p.planes_per_run - 1) / p.planes_per_run;
-  const uint64_t units = items * p.runs;
+  const uint64_t units = static_cast<uint64_t>(p.cands) * p.chunks * p.runs;
   if (units >= (1ull << 31))
     return fail(YL_ERR_UNSUPPORTED, "yl_kv_quant_store: %lld pages and heads in one call", (long long)units);
-  const unsigned grid = static_cast<unsigned>((units + kStoreThreads / 32 - 1) / (kStoreThreads / 32));
+  const unsigned grid =
+      static_cast<unsigned>(mode == kByBlock ? units : (units + kStoreThreads / 32 - 1) / (kStoreThreads / 32));
   return pick_type_dim(a->dtype, a->pool.head_dim, [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
-    auto fn = by_token ? quant_store_kernel<T, D, true> : quant_store_kernel<T, D, false>;
+    auto fn = mode == kByToken  ? quant_store_kernel<T, D, kByToken>
+              : mode == kByWarp ? quant_store_kernel<T, D, kByWarp>
+                                : quant_store_kernel<T, D, kByBlock>;
     return launch_dependent(fn, dim3(grid), dim3(kStoreThreads), 0, stream, "yl_kv_quant_store launch", p);
   });
 }
