@@ -210,3 +210,10 @@ def test_quant_pool_layout():
     C = yl.load_extension()
     assert {"StoreKVCacheQuant", "LoadKVCacheQuant", "PagedAttention", "PagedAttentionWorkspace"} <= set(dir(C))
     assert C.DeviceErrorNames(0x28000) == _abi.deverr_names(0x28000) == "NONFINITE|SCALE"
+    made = C.MakeQuantKVPool(5, 16, 3, 64, num_layers=2, device=torch.device("cpu"))
+    for a, b in zip(made, pool):
+        assert a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
+        assert torch.equal(a.float(), b.float())
+    assert C.MakeQuantKVPool(5, 16, 3, 64, device=torch.device("cpu"))[2].shape == (5, 3)
+    with pytest.raises(RuntimeError, match="positive"):
+        C.MakeQuantKVPool(5, 0, 3, 64, device=torch.device("cpu"))

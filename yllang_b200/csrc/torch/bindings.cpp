@@ -63,6 +63,15 @@ PYBIND11_MODULE(_C, m) {
   m.def("QKNormRopeStoreKV", &QKNormRopeStoreKV, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("k_cache"),
         py::arg("v_cache"), py::arg("indices"), py::arg("opts"), py::arg("q_out"));
 
+  m.def(
+      "MakeQuantKVPool",
+      [](int64_t num_pages, int64_t page_size, int64_t num_kv_heads, int64_t head_dim, int64_t num_layers,
+         const torch::Device &device) {
+        const QuantKVPool p = MakeQuantKVPool(num_pages, page_size, num_kv_heads, head_dim, num_layers, device);
+        return std::make_tuple(p.k, p.v, p.k_scale, p.v_scale);
+      },
+      py::arg("num_pages"), py::arg("page_size"), py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("num_layers") = 0,
+      py::arg("device"), "a new 8-bit pool (k, v, k_scale, v_scale); num_layers 0 leaves the layer dimension out");
   // the page arrays are passed one by one, as the Python front end's BatchIndex holds them
   m.def(
       "StoreKVCacheQuant",
