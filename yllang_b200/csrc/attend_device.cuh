@@ -90,6 +90,25 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool v
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool valid) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
 }
+// 16 bytes, or zeros where !valid.  Written out, so that the load stays in
+// flight until its value is used: a conditional expression around __ldg waited
+// for it on the spot (8-bit prompt of 8k tokens 690 -> 665 us).
+__device__ __forceinline__ uint4 ldg128_if(const void *src, bool valid) {
+  uint4 v;
+  asm volatile(
+      "{\n"
+      ".reg .pred q;\n"
+      "setp.ne.u32 q, %5, 0;\n"
+      "mov.u32 %0, 0;\n"
+      "mov.u32 %1, 0;\n"
+      "mov.u32 %2, 0;\n"
+      "mov.u32 %3, 0;\n"
+      "@q ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+      "}\n"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(src), "r"(static_cast<uint32_t>(valid)));
+  return v;
+}
 // Arrive on `bar` (no count added) once this thread's earlier cp.async have landed.
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");

@@ -10,7 +10,8 @@
 // * Warps 16-23 load: they gather rows of K and V by page, in tiles of KT tokens,
 //   and leave them 16-bit and swizzled in a ring of two stages.  16-bit pools
 //   are copied asynchronously; the codes of an 8-bit pool are converted on the
-//   way to fp16, which holds every e4m3 value.  K's scales, relative to the
+//   way to fp16, which holds every e4m3 value (K's wait for it in shared memory
+//   while the tile before is converted, V's in registers).  K's scales, relative to the
 //   largest of the tile, are multiplied in (exact for powers of two); the tile's
 //   largest goes to the scores as one factor.  V's are multiplied in relative to
 //   a reference that changes only when a tile's largest passes 64 times it, when
@@ -26,8 +27,19 @@
 //   an 8-bit pool become fp16 by a power of two per row), then per tile of keys
 //   read S once and write the weights over it in 16 bits.  The weights refer to
 //   an earlier tile's maximum: that is looked at again, and the row's accumulator
-//   rescaled, only where a sum of weights shows that one may have grown past
-//   2^8 (fp16 weights are kept times 2^3).
+//   rescaled, only where half a row's sum of weights passes 2^15, so that every
+//   weight fits fp16; weights are kept times 2^3 there, which puts fp16's
+//   smallest numbers 2^-27 below the largest weight of a row that moved.
+//
+// What bounds it: the products are 4 * 128 * 128 * head_dim flops per row tile
+// and key tile, 2,118 cycles for both row tiles at head_dim 128 when nothing else
+// runs; a tile takes about 3,850 cycles in the steady state of a 16-bit pool (an
+// 8k prompt of 32 heads: 518 us, 1,060 TFLOP/s, 0.65 of the library's measured
+// rate) and 4,900 of an 8-bit one (665 us).  The rest is the chain from a score
+// product through the softmax to the value product, which the two row tiles
+// cover only in part, and for 8-bit pools the conversion.  Masked tiles cost
+// about 1,000 cycles more, an item's start and end about 7,000: a window of 1k
+// keys has ten tiles per item, two of them masked, and runs at 0.38.
 //
 // Only tiles that some row does not see in full are masked; in those, infinities
 // and NaN of V are zeroed as they are loaded and reported to the rows that see
@@ -49,7 +61,6 @@ constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int kTileThreads = 256;  // softmax threads of a row tile
 constexpr int kStages = 2;  // of K, and of V
 constexpr int kInfos = 4;   // descriptions of tiles: one is read until the tile's values are used up
-constexpr float kMoveBy = 8.f;    // log2 of how far weights may pass 1 before their reference moves
 constexpr float kMost = 32768.f;  // sum of weights of half a row, lift included, above which they are looked at again
 constexpr float kMaxRatio = 64.f; // of a V scale to the reference
 
@@ -62,7 +73,8 @@ struct Shape {
   static constexpr int kRows = 128 * kQTiles;
   static constexpr int kQBytes = 128 * D * 2;       // one row tile
   static constexpr int kKVBytes = kKT * D * 2;      // K or V of a stage
-  static constexpr int kSmem = kQTiles * kQBytes + 2 * kStages * kKVBytes + kHeader + 1024;
+  static constexpr int kRaw = kKT * D;              // codes of a tile of K
+  static constexpr int kSmem = kQTiles * kQBytes + 2 * kStages * kKVBytes + kHeader + 1024;  // without kRaw
   static constexpr uint32_t kS = 0;    // tensor memory columns: S of tile w at w * kKT
   static constexpr uint32_t kO = 256;  // O of tile w at kO + w * D
 };
@@ -261,7 +273,7 @@ __device__ __forceinline__ uint32_t swizzled(int r, int c) {
 // Each thread looks up one token of a tile: its page id two tiles ahead, the
 // page's scales one tile ahead.
 template <typename T, int D, bool Q8>
-__device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint8_t *kv) {
+__device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint8_t *kv, uint8_t *raw) {
   using S = Shape<D>;
   constexpr int KT = S::kKT;
   constexpr bool BF = std::is_same<T, Bf16>::value && !Q8;
@@ -291,6 +303,40 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
   int page0 = more0 ? page_of(plan(0)) : kNone, page1 = more1 ? page_of(plan(1)) : kNone;
   float ks0 = 0.f, vs0 = 0.f;
   if (more0) scales_of(plan(0), page0, ks0, vs0);
+  // where the rows of tile u are, for all threads
+  auto place = [&](uint32_t u, int page) {
+    const Plan &t = plan(u);
+    int64_t off = -1;
+    if (good(page)) {
+      const int pos = t.base + tid;
+      off = static_cast<int64_t>(page) * p.page_stride +
+            static_cast<int64_t>(pos - static_cast<int>(p.by_page.div(pos)) * p.page_size) * p.slot_stride +
+            t.head * p.head_stride;
+    } else if (page != kNone) {
+      raise_deverr(p.error_word, page == kNoEntry ? YL_DEVERR_INDICES_CAP : YL_DEVERR_PAGE_RANGE);
+    }
+    if (tid < KT) sh->offset[u & 1][tid] = off;
+    const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
+    if (lane == 0 && warp * 32 < KT) sh->valid[u & 1][warp] = ok;
+  };
+  constexpr int CH = D * (Q8 ? 1 : 2) / 16;    // 16-byte chunks of a token's head row
+  constexpr int STEP = kLoadThreads / CH;      // rows of one pass of the threads
+  constexpr int PER = KT / STEP;               // chunks of a thread
+  const int c = tid % CH, r0 = tid / CH;
+  // K's codes of tile u, each thread's chunks into its own places of `raw`
+  const uint32_t mine = smem_addr(raw) + tid * 16;
+  auto fetch_keys = [&](uint32_t u) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int64_t o = sh->offset[u & 1][r0 + i * STEP];
+      cp_async16(mine + i * kLoadThreads * 16, p.kv[0] + (o >= 0 ? o + c * 16 : 0), o >= 0);
+    }
+  };
+  if (more0) {
+    place(0, page0);
+    load_barrier(true);
+    if (Q8) fetch_keys(0);
+  }
   float value = 0.f;  // reference of V's scales
   bool lost = false;  // a wait gave up: the next barrier ends all of them
   uint32_t used = 0;
@@ -304,18 +350,6 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
     if (more1) scales_of(plan(used + 1), page1, ks1, vs1);
     const Plan &t0 = plan(used);
 
-    int64_t off = -1;
-    if (good(page0)) {
-      const int pos = t0.base + tid;
-      off = static_cast<int64_t>(page0) * p.page_stride +
-            static_cast<int64_t>(pos - static_cast<int>(p.by_page.div(pos)) * p.page_size) * p.slot_stride +
-            t0.head * p.head_stride;
-    } else if (page0 != kNone) {
-      raise_deverr(p.error_word, page0 == kNoEntry ? YL_DEVERR_INDICES_CAP : YL_DEVERR_PAGE_RANGE);
-    }
-    if (tid < KT) sh->offset[par][tid] = off;
-    const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
-    if (lane == 0 && warp * 32 < KT) sh->valid[par][warp] = ok;
     if (Q8) {
       float ktop = ks0, vtop = vs0;
 #pragma unroll
@@ -329,6 +363,7 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
       }
     }
     load_barrier(true);
+    if (more1) place(used + 1, page1);  // (nobody reads the tile before this one's places any more)
     float key = 1.f, move = 1.f;
     if (t0.flags & kFirst) value = Q8 ? 0.f : 1.f;
     if (Q8) {
@@ -356,17 +391,12 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
     const bool edge = all != 0xffffffffu || t0.base + KT - 1 > t0.first_pos ||
                       (p.window > 0 && t0.base <= t0.last_pos - p.window && t0.base + KT > p.sinks);
     const uint32_t sk = smem_addr(kv + stage * 2 * S::kKVBytes), sv = sk + S::kKVBytes;
-    constexpr int CH = D * (Q8 ? 1 : 2) / 16;    // 16-byte chunks of a token's head row
-    constexpr int STEP = kLoadThreads / CH;      // rows of one pass of the threads
-    constexpr int PER = KT / STEP;               // chunks of a thread
-    const int c = tid % CH, r0 = tid / CH;
     uint4 w[Q8 ? PER : 1];
-    if (Q8) {  // K's codes are on their way before the stage is free
+    if (Q8) {  // V's codes are on their way before K is converted
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int64_t o = sh->offset[par][r0 + i * STEP];
-        w[i] = make_uint4(0, 0, 0, 0);
-        if (o >= 0) w[i] = __ldg(reinterpret_cast<const uint4 *>(p.kv[0] + o + c * 16));
+        w[i] = ldg128_if(p.kv[1] + o + c * 16, o >= 0);
       }
     }
     // K's previous tile of this stage is used up; V's is waited for behind K
@@ -389,9 +419,8 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
     if (lane == 0) mbar_arrive(&sh->plan_empty[used % kPlans]);  // (every thread has read it)
 
     if (Q8) {
-      auto convert = [&](int i, int r, int kv_i) {
+      auto convert = [&](const uint32_t (&x)[4], int r, int kv_i) {
         const uint32_t ratio = sh->ratio[par][kv_i][r];
-        const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
         uint32_t y[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -408,19 +437,25 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
         sts128(at + swizzled<KT>(r, 2 * c), y[0], y[1], y[2], y[3]);
         sts128(at + swizzled<KT>(r, 2 * c + 1), y[4], y[5], y[6], y[7]);
       };
+      cp_async_wait_all();
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int r = r0 + i * STEP;
-        convert(i, r, 0);
-        const int64_t o = sh->offset[par][r];
-        w[i] = make_uint4(0, 0, 0, 0);
-        if (o >= 0) w[i] = __ldg(reinterpret_cast<const uint4 *>(p.kv[1] + o + c * 16));
+        uint32_t x[4];
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                     : "r"(mine + i * kLoadThreads * 16)
+                     : "memory");
+        convert(x, r0 + i * STEP, 0);
       }
       fence_to_async();
       mbar_arrive(&sh->k_full[stage]);
+      if (more1) fetch_keys(used + 1);  // on their way while V is converted
       lost = !wait_or_report(p, &sh->v_empty[stage], phase);
 #pragma unroll
-      for (int i = 0; i < PER; ++i) convert(i, r0 + i * STEP, 1);
+      for (int i = 0; i < PER; ++i) {
+        const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        convert(x, r0 + i * STEP, 1);
+      }
       fence_to_async();
       mbar_arrive(&sh->v_full[stage]);
     } else {
@@ -802,7 +837,9 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
       }
       if (again) {
         // Else, and for the first tile, the maximum first; rows whose weights would
-        // pass 2^kMoveBy take it as their reference.
+        // pass 1 take it as their reference, all of them while the tile is here:
+        // when only weights above 2^8 moved it, some row came back at every third
+        // tile of scores with a spread of tens.
         float top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < C / 32; ++k) {
@@ -818,7 +855,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
         *mine = top;
         tile_barrier(w, false);
         top = fmaxf(top, *other) * c;
-        if (top > m + kMoveBy) {
+        if (top > m) {
           const float f = fast_exp2(m - top);
           m = top;
           l *= f;
@@ -914,7 +951,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     softmax_rows<T, D, Q8>(p, sh, q, warp >> 3, warp >> 2 & 1);
   } else if (warp < kSoftmaxWarps + kLoadWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    load_tiles<T, D, Q8>(p, sh, kv);
+    load_tiles<T, D, Q8>(p, sh, kv, reinterpret_cast<uint8_t *>(sh) + kHeader);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == kThreads / 32 - 3) plan_tiles<D>(p, sh);
@@ -933,12 +970,13 @@ int launch_prefill(AttnParams &p, const yl_paged_attention_args *a, cudaStream_t
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     constexpr bool Q8 = decltype(q8)::value;
-    const int rc = allow_smem(reinterpret_cast<const void *>(prefill_kernel<T, D, Q8>), Shape<D>::kSmem);
+    constexpr int smem = Shape<D>::kSmem + (Q8 ? Shape<D>::kRaw : 0);
+    const int rc = allow_smem(reinterpret_cast<const void *>(prefill_kernel<T, D, Q8>), smem);
     if (rc != YL_OK) return rc;
     // no more items than full row tiles of the batch and one more per sequence
     const int64_t items = (a->num_tokens * p.group / Shape<D>::kRows + a->batch_size) * p.heads;
     return launch_dependent(prefill_kernel<T, D, Q8>, dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count()))),
-                            dim3(kThreads), Shape<D>::kSmem, stream, "yl_paged_attention launch", p);
+                            dim3(kThreads), smem, stream, "yl_paged_attention launch", p);
   };
   auto kind = [&](auto t, auto d) {
     return a->kv_dtype == YL_KV_E4M3 ? go(t, d, std::true_type{}) : go(t, d, std::false_type{});
