@@ -512,6 +512,7 @@ YL_API int yl_kv_quant_load(const yl_quant_load_args *args, cudaStream_t stream)
  * Where a query sees a V row that holds an infinity or NaN, any element of
  * its result may be NaN.  Any number of new tokens per sequence, none
  * included, and any page size.  Rows of o behind qo_indptr[B] stay as they were.
+ * o must not overlap q or the pool.
  *
  * A seen page outside [0, num_pages) sets YL_DEVERR_PAGE_RANGE and counts as
  * not seen, entries past kv_indices_capacity YL_DEVERR_INDICES_CAP likewise;

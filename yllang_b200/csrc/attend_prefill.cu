@@ -296,8 +296,9 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
   // plan u, waited for; the plans behind the last tile's stay unread
   auto plan = [&](uint32_t u) -> const Plan & { return sh->plan[u % kPlans]; };
   auto planned = [&](uint32_t u) { return warp_wait(p, &sh->plan_full[u % kPlans], u / kPlans & 1); };
-  bool more0 = planned(0) && plan(0).live != 0;
-  const bool early = !more0 || planned(1);
+  const bool begun = planned(0);
+  bool more0 = begun && plan(0).live != 0;
+  const bool early = begun && (!more0 || planned(1));
   bool more1 = more0 && early && plan(1).live != 0;
   if (!load_barrier(early)) return;  // all of them, or none
   int page0 = more0 ? page_of(plan(0)) : kNone, page1 = more1 ? page_of(plan(1)) : kNone;

@@ -13,7 +13,13 @@
 // the token-major input.  A warp finds its page once (a 32-way search over the
 // batch) and walks its planes.
 //
-// Algorithmic bytes per element: 2 read + 1 written, so both are bound by HBM.
+// Algorithmic bytes per element: 2 read + 1 written for the store, 1 read + 2
+// written for the load, so HBM bounds both.  Measured, bf16 rows of 8 heads of
+// 128: a prompt step of 64 sequences, 32 layers, 269 us, 6.75 TB/s, as fast as a
+// plain copy; a decode step of 256 sequences, 32 layers, 23 us, 2.2 TB/s (bound
+// by one chain of loads: batch arrays, page, scale, rows); 131,072 tokens of one
+// layer read back in 156 us, 5.2 TB/s, where two bytes in three are writes and
+// a fill of the same memory reaches 3.9 TB/s.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -314,6 +320,10 @@ __device__ __noinline__ void store_rows_twice(const QuantStoreParams &p, const T
 // tokens): four warps share a page, up to 64 rows in registers, and exchange
 // their maxima; of longer pages the rows are read twice.  They are kernels of
 // their own, since the registers of one would cost the other's warps in flight.
+// Both sides of each rule, 32 layers of 8 heads of 128: 256 sequences of one token
+// by token 22.6 us, by warp 29.4; 64 prompts in pages of 16 by warp 269 us, by
+// block 659; pages of 8 by warp 351, by block 1,208; pages of 64 by block 274,
+// by warp 528.
 enum StoreMode { kByToken, kByWarp, kByBlock };
 
 template <typename T, int D>

@@ -545,7 +545,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     tokens of one sequence where the caller knows it (1 for a decode batch),
     which saves launches; sequences of more are skipped with
     DEVERR_TOKEN_COUNT.  Rows behind the last sequence are left as they were
-    (uninitialised in a new output).  workspace: uint8 tensor of at least
+    (uninitialised in a new output); out must not overlap q.  workspace: uint8 tensor of at least
     paged_attention_workspace(...) bytes; by default the call allocates it.
     Calls that may overlap on the GPU need a workspace each."""
     got = _run(_front_end().PagedAttention, "paged_attention", q.device, stream, error_word,
