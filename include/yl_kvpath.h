@@ -445,8 +445,8 @@ typedef struct yl_quant_pool {
  * Pages outside [0, num_pages) set YL_DEVERR_PAGE_RANGE, entries past
  * kv_indices_capacity YL_DEVERR_INDICES_CAP, rows past num_tokens
  * YL_DEVERR_TOKEN_COUNT, more new tokens than the sequence's pages hold
- * YL_DEVERR_ROW_OVERFLOW; each skips those rows.  Rows behind qo_indptr[B] are
- * not read.  A page that two sequences of one call write is outside the
+ * YL_DEVERR_ROW_OVERFLOW; each skips those rows.  Rows behind qo_indptr[B] have
+ * no effect.  A page that two sequences of one call write is outside the
  * contract.  Row pointers and strides of k and v are multiples of 16 bytes,
  * codes of 8.
  */

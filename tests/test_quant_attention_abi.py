@@ -53,6 +53,8 @@ POOL_ERRORS = [
     (dict(pool_head_dim=96), _abi.YL_ERR_UNSUPPORTED),
     (dict(pool_num_pages=1 << 27), _abi.YL_ERR_UNSUPPORTED),  # 2^31 slots
     (dict(pool_num_pages=1 << 31), _abi.YL_ERR_UNSUPPORTED),
+    (dict(pool_num_layers=1 << 30), _abi.YL_ERR_UNSUPPORTED),
+    (dict(pool_num_heads=2 ** 31 - 1), _abi.YL_ERR_UNSUPPORTED),
     (dict(pool_k_codes=0), _abi.YL_ERR_NULL_ARG),
     (dict(pool_v_scale=0), _abi.YL_ERR_NULL_ARG),
     (dict(pool_slot_stride=64), _abi.YL_ERR_BAD_SIZE),

@@ -233,6 +233,7 @@ __device__ __forceinline__ void store_planes(const QuantStoreParams &p, const To
       old[b] = p.pool.scale[kv][layer * p.pool.scale_layer_stride + pg.page * p.pool.scale_page_stride +
                                 h * p.pool.scale_head_stride];
   }
+  __syncwarp();  // every lane has the old scales
 #pragma unroll
   for (int b = 0; b < PB; ++b) {
     const int plane = plane0 + b, kv = plane & 1, layer = plane >> 1;
@@ -284,6 +285,9 @@ __device__ __noinline__ void store_rows_twice(const QuantStoreParams &p, const T
   const int h = active ? head : 0;
   const int64_t stride = p.row_stride[kv];
   const char *src = row_of<D>(p, pg.row0, plane, h, lane);
+  float *sc = p.pool.scale[kv] + layer * p.pool.scale_layer_stride + pg.page * p.pool.scale_page_stride +
+              h * p.pool.scale_head_stride;
+  const float old = active && pg.held > 0 ? *sc : 0.f;
   float amax = 0.f;
   bool bad = false;
   if (active)
@@ -296,15 +300,12 @@ __device__ __noinline__ void store_rows_twice(const QuantStoreParams &p, const T
 #pragma unroll
   for (int d = LPR / 2; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
   if (bad) raise_deverr(p.error_word, YL_DEVERR_NONFINITE);
+  __syncwarp();  // every lane has the old scale
   if (!active) return;
   uint8_t *dst = p.pool.codes[kv] + layer * p.pool.layer_stride + pg.page * p.pool.page_stride + h * p.pool.head_stride +
                  sub * 8;
-  float *sc = p.pool.scale[kv] + layer * p.pool.scale_layer_stride + pg.page * p.pool.scale_page_stride +
-              h * p.pool.scale_head_stride;
-  const float old = pg.held > 0 ? *sc : 0.f;
   const NewScale n = new_scale(p, amax, pg.held, old, sub == 0);
   if (n.ratio != 1.f) requantise(dst, p.pool.slot_stride, 0, pg.held, 1, n.ratio);
-  __syncwarp(__activemask());  // every lane has the old scale
   if (n.write && sub == 0) *sc = n.scale;
   const float inv = 1.f / n.scale;  // exact for a power of two
   dst += pg.held * p.pool.slot_stride;
@@ -553,6 +554,8 @@ int check_pool(const yl_quant_pool &q, int align, const char *who, QuantPool &ou
   if (q.page_size < 1) return bad(YL_ERR_BAD_SIZE, "page_size=%lld < 1", q.page_size);
   if (q.num_heads < 1) return bad(YL_ERR_BAD_SIZE, "num_heads=%lld < 1", q.num_heads);
   if (q.num_pages < 1) return bad(YL_ERR_BAD_SIZE, "num_pages=%lld < 1", q.num_pages);
+  if (q.num_layers >= 1 << 24 || q.num_heads >= 1 << 24)
+    return bad(YL_ERR_UNSUPPORTED, "num_layers=%lld and num_heads must be below 2^24", q.num_layers);
   if (q.head_dim != 64 && q.head_dim != 128 && q.head_dim != 256)
     return bad(YL_ERR_UNSUPPORTED, "head_dim=%lld must be 64, 128 or 256", q.head_dim);
   if (q.num_pages >= (1ll << 31) || q.num_pages * q.page_size >= (1ll << 31))

@@ -503,7 +503,7 @@ def store_kv_cache_quant(k: torch.Tensor, v: torch.Tensor, pool: QuantKVPool, in
     k, v: bf16 or fp16 [N, H*D] (or [N, H, D]) rows of one layer, or
     [L, N, H*D] ([L, N, H, D]) for an all-layer pool, in the order of the page
     arrays that build_index gave (rows qo_indptr[i] .. qo_indptr[i+1] are
-    sequence i's new tokens; rows behind the last are not read).  Each page
+    sequence i's new tokens; rows behind the last have no effect).  Each page
     and head has one power-of-two scale; where new tokens need a larger one,
     the page's earlier tokens take it too (see yl_kv_quant_store).  Pages that
     two sequences of one call write are outside the contract.  An infinity is
