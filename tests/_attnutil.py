@@ -106,7 +106,7 @@ def attention_bound(want, spread, reach, dtype, weights, head_dim):
     rounding; the weights' one rounding to `weights`; and fp32 arithmetic of
     the scores, off by (head_dim + 4) half steps of 2^-24 times the sum of
     |q| |k|, which changes a weight and the sum of weights by that much each,
-    with 2^-21 for the exponential and the sums; weights more than 2^-24 below
-    the largest (2^-39 with the lift of the fp16 ones) may vanish."""
+    with 2^-21 for the exponential and the sums; fp16 weights more than 2^-24
+    below the largest may vanish (with their lift, 2^-27 and less)."""
     delta = 2 * reach * (head_dim + 4) * 2.0 ** -24 + 2.0 ** -20
     return HALF_STEP[dtype] * want.abs() + (HALF_STEP[weights] + 2 * delta) * spread * (1 + 2.0 ** -8) + 1e-7

@@ -351,3 +351,54 @@ def test_a_batch_of_thousands(cuda):
     prior = [(i * 7) % 4 for i in range(9000)]
     _run(cuda, prior, new, H=1, G=1, D=64, ps=4, pad=2, kv="16", dtype=torch.float16)
     _run(cuda, prior, new, H=1, G=1, D=64, ps=4, pad=2, hint=False)
+
+
+def test_padded_batch_of_empty_sequences(cuda):
+    """Rows of padding only: no page, an empty kv_indices, nothing written."""
+    H, G, D, ps, P = 2, 2, 64, 16, 4
+    pool = yl.quant_kv_pool(P, ps, H, D, device=cuda)
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32, device=cuda)  # noqa: E731
+    idx = yl.BatchIndex(i32(3), i32(0), i32(2), i32(3), None)
+    rows = torch.ones(5, H, D, dtype=torch.bfloat16, device=cuda)
+    q = torch.ones(5, H * G, D, dtype=torch.bfloat16, device=cuda)
+    err, out = i32(1), torch.full_like(q, 7.0)
+    yl.store_kv_cache_quant(rows, rows, pool, idx, error_word=err)
+    _direct(q, pool.k, pool.v, pool.k_scale, pool.v_scale, idx, out=out, error_word=err)
+    assert int(err.item()) == 0 and not bool((pool.k.float() != 0).any()) and bool((out == 7.0).all())
+    assert bool((pool.k_scale == 1).all())
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_queries_as_heads_major_memory(cuda, new):
+    """q and out in [heads, tokens, D] memory, the strides of rows below those of heads."""
+    H, G, D, ps, P = 2, 4, 128, 16, 60
+    prior = [200, 33]
+    idx, pages = make_index(prior, [new, new], ps, P, 1)
+    (k, v, ks, vs), (kx, vx) = _pool(P, ps, H, D, torch.bfloat16, "e4m3", cuda, 2)
+    q = torch.randn(2 * new, H * G, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    mem = q.to(cuda).transpose(0, 1).contiguous().transpose(0, 1)
+    out = torch.zeros_like(q.transpose(0, 1).contiguous(), device=cuda).transpose(0, 1)
+    got = _direct(mem, k, v, ks, vs, idx, out=out)
+    want, spread, reach = attention_reference(q, kx, vx, prior, [new, new], pages)
+    _check(got, want, spread, reach, torch.bfloat16, "e4m3", D)
+
+
+@pytest.mark.parametrize("kv", ["e4m3", "16"])
+def test_scores_that_fall_and_rise(cuda, kv):
+    """Keys whose loudness grows along the sequence, then falls: the reference
+    moves at nearly every tile, in decode and in prefill."""
+    H, G, D, ps, P = 1, 4, 128, 16, 40
+    for prior, new in (([600], [1]), ([300], [301])):
+        idx, pages = make_index(prior, new, ps, P, 1)
+        (k, v, ks, vs), (kx, vx) = _pool(P, ps, H, D, torch.float16, kv, cuda, 2)
+        for j, page in enumerate(pages[0]):
+            f = 2.0 ** (min(j, 37 - j) // 6 - 2)
+            if kv == "e4m3":
+                ks[page] *= f
+            else:
+                k[page] *= f
+            kx[page] *= f
+        q = torch.randn(sum(new), H * G, D, generator=torch.Generator().manual_seed(3)).to(torch.float16)
+        got = _direct(q.to(cuda), k, v, ks, vs, idx)
+        want, spread, reach = attention_reference(q, kx, vx, prior, new, pages)
+        _check(got, want, spread, reach, torch.float16, kv, D)

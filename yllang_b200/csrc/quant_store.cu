@@ -631,7 +631,8 @@ extern "C" int yl_kv_quant_store(const yl_quant_store_args *a, cudaStream_t stre
   QuantStoreParams p;
   int rc = check_pool(a->pool, 8, who, p.pool);
   if (rc != YL_OK) return rc;
-  if (!a->k || !a->v || !a->kv_indptr || !a->kv_last_page_len || !a->qo_indptr || !a->kv_indices)
+  if (!a->k || !a->v || !a->kv_indptr || !a->kv_last_page_len || !a->qo_indptr ||
+      (!a->kv_indices && a->kv_indices_capacity > 0))
     return fail(YL_ERR_NULL_ARG, "yl_kv_quant_store: k, v and the page arrays must be non-NULL");
   rc = check_rows(a->k, a->v, a->k_row_stride, a->v_row_stride, a->k_layer_stride, a->v_layer_stride, a->pool, who);
   if (rc != YL_OK) return rc;
