@@ -47,6 +47,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cstdint>
 
 #include "attend_device.cuh"
@@ -788,7 +789,12 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
       wait(&sh->s_full[w], waits++ & 1);  // (issued behind the tile's description)
       tc_fence_after();
       const TileInfo *info = &sh->tile[used % kInfos];
-      const float c = coef * info->key;
+      // Kept a normal number: a zero row's factor is scale_log2 * 2^-126, and times
+      // a K scale of 2^-22 it would be 0, which times the -inf of a hidden column
+      // is no number.  (A row's scores are at most 2^18 times the factor, so the
+      // smallest normal one stands for all below it; the largest, so that 0 times
+      // it stays 0.)
+      const float c = Q8 ? fminf(fmaxf(coef * info->key, FLT_MIN), FLT_MAX) : coef;
       float factor = info->move;
       if (edge) look_back(used - 1);  // (the scores' products were issued behind its values')
       edge = info->edge != 0;
