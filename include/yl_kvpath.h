@@ -445,10 +445,11 @@ typedef struct yl_quant_pool {
  * Pages outside [0, num_pages) set YL_DEVERR_PAGE_RANGE, entries past
  * kv_indices_capacity YL_DEVERR_INDICES_CAP, rows past num_tokens
  * YL_DEVERR_TOKEN_COUNT, more new tokens than the sequence's pages hold
- * YL_DEVERR_ROW_OVERFLOW; each skips those rows.  Rows behind qo_indptr[B] have
- * no effect.  A page that two sequences of one call write is outside the
- * contract.  Row pointers and strides of k and v are multiples of 16 bytes,
- * codes of 8.
+ * YL_DEVERR_ROW_OVERFLOW; each skips those rows.  Rows in front of qo_indptr[0]
+ * and behind qo_indptr[B] have no effect, so a slice of a batch's page arrays is
+ * a batch over the same rows.  A page that two sequences of one call write is
+ * outside the contract.  Row pointers and strides of k and v are multiples of 16
+ * bytes, codes of 8.
  */
 typedef struct yl_quant_store_args {
   yl_quant_pool pool;
@@ -511,8 +512,8 @@ YL_API int yl_kv_quant_load(const yl_quant_load_args *args, cudaStream_t stream)
  * anything (a window's pages can be given back while their entries stay).
  * Where a query sees a V row that holds an infinity or NaN, any element of
  * its result may be NaN.  Any number of new tokens per sequence, none
- * included, and any page size.  Rows of o behind qo_indptr[B] stay as they were.
- * o must not overlap q or the pool.
+ * included, and any page size.  Rows of o in front of qo_indptr[0] and behind
+ * qo_indptr[B] stay as they were.  o must not overlap q or the pool.
  *
  * A seen page outside [0, num_pages) sets YL_DEVERR_PAGE_RANGE and counts as
  * not seen, entries past kv_indices_capacity YL_DEVERR_INDICES_CAP likewise;

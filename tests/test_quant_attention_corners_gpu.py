@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import yllang_b200 as yl
-from _attnutil import attention_reference, make_index
+from _attnutil import attention_reference, make_index, store_reference
 from test_paged_attention_gpu import _check, _pool
 
 pytestmark = pytest.mark.gpu
@@ -44,3 +44,41 @@ def test_rows_whose_scores_vanish_give_the_mean_of_the_values(cuda, dtype, D, ki
     assert int(err.item()) == 0
     want, spread, reach = attention_reference(q, kx, vx, prior, new, pages)
     _check(got, want, spread, reach, dtype, "e4m3", D)
+
+
+@pytest.mark.parametrize("batch", [([0, 17, 5, 200, 3, 14, 33, 1], [1] * 8),
+                                   ([0, 7, 16, 31, 0, 64, 3], [50, 1, 16, 2, 1, 0, 13])], ids=["decode", "ragged"])
+@pytest.mark.parametrize("ps", [1, 4, 16, 64])
+@pytest.mark.parametrize("part", [(1, 3), (3, 7), (0, 4), (5, 7), (5, 6)])
+def test_a_slice_of_a_batch_over_all_of_its_rows(cuda, batch, ps, part):
+    """Page arrays of the sequences [lo, hi) beside the rows of the whole batch:
+    those sequences' tokens and nothing else are stored, and attended."""
+    lo, hi = part
+    H, G, D = 3, 2, 64
+    prior, new = batch
+    P = sum(-(-(a + b) // ps) for a, b in zip(prior, new)) + 2
+    whole, pages = make_index(prior, new, ps, P, 1)
+    idx = yl.BatchIndex(whole.kv_indptr[lo:hi + 1], whole.kv_indices, whole.kv_last_page_len[lo:hi],
+                        whole.qo_indptr[lo:hi + 1], None)
+    first, last = sum(new[:lo]), sum(new[:hi])
+    g = torch.Generator().manual_seed(ps)
+    x = torch.randn(2, sum(new), H, D, generator=g) * torch.exp2(torch.randint(-3, 4, (2, sum(new), 1, 1), generator=g))
+    x = x.to(torch.float16)
+    pool = yl.quant_kv_pool(P, ps, H, D, device=cuda)
+    want = [t.double().cpu() for t in pool]
+    for i in range(2):
+        store_reference(x[i, first:last].double(), want[i], want[2 + i], prior[lo:hi], new[lo:hi], pages[lo:hi], ps)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    yl.store_kv_cache_quant(x[0].to(cuda), x[1].to(cuda), pool, idx, error_word=err)
+    assert int(err.item()) == 0
+    for got, w in zip(pool, want):
+        assert torch.equal(got.double().cpu(), w)
+    q = torch.randn(sum(new), H * G, D, generator=g).to(torch.float16)
+    out = torch.full_like(q, 7.0, device=cuda)
+    yl.paged_attention(q.to(cuda), pool.k, pool.v, idx, k_scale=pool.k_scale, v_scale=pool.v_scale, out=out,
+                       error_word=err)
+    assert int(err.item()) == 0
+    kx, vx = (w * s[:, None, :, None] for w, s in zip(want[:2], want[2:]))
+    o, spread, reach = attention_reference(q[first:last], kx, vx, prior[lo:hi], new[lo:hi], pages[lo:hi])
+    _check(out[first:last], o, spread, reach, torch.float16, "e4m3", D)
+    assert bool((out[:first] == 7.0).all()) and bool((out[last:] == 7.0).all())

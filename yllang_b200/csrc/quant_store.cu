@@ -102,7 +102,7 @@ __device__ __forceinline__ Touched find_page(const QuantStoreParams &p, uint32_t
   if (BY_TOKEN) {
     const int64_t t = static_cast<int64_t>(cand) - q0;
     const int64_t pos = prior + t;
-    if (t >= fresh) return r;  // a row behind the last sequence
+    if (t < 0 || t >= fresh) return r;  // a row in front of the first sequence, or behind the last
     if (prior < 0 && t == 0 && report) raise_deverr(p.error_word, YL_DEVERR_ROW_OVERFLOW);
     if (pos < 0 || (t > 0 && pos % ps != 0)) return r;
     ord = pos / ps;

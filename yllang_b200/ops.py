@@ -503,7 +503,8 @@ def store_kv_cache_quant(k: torch.Tensor, v: torch.Tensor, pool: QuantKVPool, in
     k, v: bf16 or fp16 [N, H*D] (or [N, H, D]) rows of one layer, or
     [L, N, H*D] ([L, N, H, D]) for an all-layer pool, in the order of the page
     arrays that build_index gave (rows qo_indptr[i] .. qo_indptr[i+1] are
-    sequence i's new tokens; rows behind the last have no effect).  Each page
+    sequence i's new tokens; rows in front of the first and behind the last
+    have no effect, so the arrays may be a slice of a batch's).  Each page
     and head has one power-of-two scale; where new tokens need a larger one,
     the page's earlier tokens take it too (see yl_kv_quant_store).  Pages that
     two sequences of one call write are outside the contract.  An infinity is
@@ -544,8 +545,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     sm_scale: 1 / sqrt(D) by default.  max_new_len: an upper bound of the new
     tokens of one sequence where the caller knows it (1 for a decode batch),
     which saves launches; sequences of more are skipped with
-    DEVERR_TOKEN_COUNT.  Rows behind the last sequence are left as they were
-    (uninitialised in a new output); out must not overlap q.  workspace: uint8 tensor of at least
+    DEVERR_TOKEN_COUNT.  Rows in front of the first sequence and behind the
+    last are left as they were (uninitialised in a new output); out must not
+    overlap q.  workspace: uint8 tensor of at least
     paged_attention_workspace(...) bytes; by default the call allocates it.
     Calls that may overlap on the GPU need a workspace each."""
     got = _run(_front_end().PagedAttention, "paged_attention", q.device, stream, error_word,
