@@ -82,3 +82,20 @@ def test_a_slice_of_a_batch_over_all_of_its_rows(cuda, batch, ps, part):
     o, spread, reach = attention_reference(q[first:last], kx, vx, prior[lo:hi], new[lo:hi], pages[lo:hi])
     _check(out[first:last], o, spread, reach, torch.float16, "e4m3", D)
     assert bool((out[:first] == 7.0).all()) and bool((out[last:] == 7.0).all())
+
+
+@pytest.mark.parametrize("batch", [([4, 0, 9], [1, 1, 1]), ([4, 0, 9], [20, 9, 1]), ([4, 0], [20, 8]), ([0, 3], [8, 16])],
+                         ids=["decode", "ragged", "two", "whole pages"])
+@pytest.mark.parametrize("ps", [1, 4, 8, 32])
+def test_store_reports_every_missing_row(cuda, batch, ps):
+    """K and V have fewer rows than the batch: the bit, and the rows that there are."""
+    H, D, P = 2, 64, 48
+    idx, _ = make_index(*batch, ps, P, 1)
+    n = sum(batch[1])
+    for rows in range(1, n + 2):
+        pool = yl.quant_kv_pool(P, ps, H, D, device=cuda)
+        err = torch.zeros(1, dtype=torch.int32, device=cuda)
+        k = torch.ones(rows, H, D, dtype=torch.bfloat16, device=cuda)
+        yl.store_kv_cache_quant(k, k, pool, idx, error_word=err)
+        written = int((pool.k.float() != 0).any(-1).any(-1).sum())
+        assert (int(err.item()), written) == (yl.DEVERR_TOKEN_COUNT if rows < n else 0, min(rows, n)), rows

@@ -412,7 +412,14 @@ __global__ void __launch_bounds__(kStoreThreads, MODE == kByToken ? 7 : 4)
   pdl_wait();  // rows and page arrays may be written by the kernel just before this one
   const uint32_t part = unit % p.chunks, rest = unit / p.chunks;
   const uint32_t cand = rest % p.cands, run = rest / p.cands;
-  if (run >= p.runs) return;
+  if (run >= p.runs) {
+    // By token the rows that k and v lack are nobody's number: the first warp
+    // behind the units, which the host leaves room for, looks for them.
+    if (MODE == kByToken && run == p.runs && cand == 0 && part == 0 && lane == 0 &&
+        __ldg(p.qo_indptr + p.batch) > p.num_tokens)
+      raise_deverr(p.error_word, YL_DEVERR_TOKEN_COUNT);
+    return;
+  }
   const int first = run * p.planes_per_run;
   const int end = min(first + static_cast<int>(p.planes_per_run), p.planes);
   const bool report = part == 0 && run == 0 && lane == 0 && (MODE != kByBlock || threadIdx.x == 0);
@@ -670,8 +677,10 @@ extern "C" int yl_kv_quant_store(const yl_quant_store_args *a, cudaStream_t stre
   const uint64_t units = static_cast<uint64_t>(p.cands) * p.chunks * p.runs;
   if (units >= (1ull << 31))
     return fail(YL_ERR_UNSUPPORTED, "yl_kv_quant_store: %lld pages and heads in one call", (long long)units);
-  const unsigned grid =
-      static_cast<unsigned>(mode == kByBlock ? units : (units + kStoreThreads / 32 - 1) / (kStoreThreads / 32));
+  constexpr int kWarps = kStoreThreads / 32;
+  const unsigned grid = static_cast<unsigned>(mode == kByBlock   ? units
+                                              : mode == kByToken ? units / kWarps + 1  // a warp beyond the units
+                                                                 : (units + kWarps - 1) / kWarps);
   return pick_type_dim(a->dtype, a->pool.head_dim, [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
