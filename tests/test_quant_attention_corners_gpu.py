@@ -99,3 +99,21 @@ def test_store_reports_every_missing_row(cuda, batch, ps):
         yl.store_kv_cache_quant(k, k, pool, idx, error_word=err)
         written = int((pool.k.float() != 0).any(-1).any(-1).sum())
         assert (int(err.item()), written) == (yl.DEVERR_TOKEN_COUNT if rows < n else 0, min(rows, n)), rows
+
+
+@pytest.mark.parametrize("kv", ["e4m3", "16"])
+@pytest.mark.parametrize("new,have", [(10, 5), (3, 1), (90, 60), (90, 3), (90, 89)])
+@pytest.mark.parametrize("window", [0, 9])
+def test_rows_that_are_there_keep_their_positions(cuda, kv, new, have, window):
+    """q and o end inside the sequence's rows: the bit, and the rows that there
+    are give what they give beside the others."""
+    H, G, D, ps, prior = 2, 2, 64, 16, 21
+    P = 12
+    idx, pages = make_index([prior], [new], ps, P, 1)
+    (k, v, ks, vs), (kx, vx) = _pool(P, ps, H, D, torch.float16, kv, cuda, 2)
+    q = torch.randn(new, H * G, D, generator=torch.Generator().manual_seed(3)).to(torch.float16)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    got = yl.paged_attention(q[:have].to(cuda), k, v, idx, k_scale=ks, v_scale=vs, window=window, sinks=2, error_word=err)
+    assert int(err.item()) == yl.DEVERR_TOKEN_COUNT
+    want, spread, reach = attention_reference(q, kx, vx, [prior], [new], pages, window, 2)
+    _check(got, want[:have], spread[:have], reach[:have], torch.float16, kv, D)

@@ -326,12 +326,12 @@ __device__ __forceinline__ void load_units(const AttnParams &p, const Place &pla
     const uint32_t valid = __ballot_sync(0xffffffffu, ok);
     // this unit's description, before the state moves on
     const bool is_first = u == 0 || tile == 0, ends = tile == w.tiles - 1;
-    const int rows = s.fresh * p.group, row0 = rt * kRows, pos0 = s.total - s.fresh, q0 = s.q0, u_base = base, u_head = head;
+    const int rows = s.fresh * p.group, row0 = rt * kRows, pos0 = s.first, q0 = s.q0, u_base = base, u_head = head;
     const int64_t seg = begin + (static_cast<int64_t>(head) * w.row_tiles + rt) * w.tiles;  // its first unit in the line
     int flags = is_first ? kFirst : 0;
     if (ends || u == count - 1) flags |= kLast;
     if (ends && seg >= first) flags |= kWhole;
-    const int last_pos = s.total - 1, end = base + cnt - 1;
+    const int last_pos = max(s.first + s.fresh - 1, -1), end = base + cnt - 1;
     const bool all = end <= pos0 && (p.window == 0 || base > last_pos - p.window || end < p.sinks);
     if (s.fresh > 1 && !all) flags |= kRagged;
     if (u == 0 && quarter == 0 && lane == 0) {

@@ -34,10 +34,11 @@ struct AttnParams {
 
 constexpr int64_t kMaxTotal = 1ll << 30;  // tokens of one sequence
 
-// A sequence of the batch.  Its query t is at position total - fresh + t.
+// A sequence of the batch.  Its query t is at position first + t.
 struct Seq {
   int q0;     // first row of q and o
-  int fresh;  // new tokens
+  int fresh;  // new tokens that have rows in q and o
+  int first;  // position of the first new token; below 0 where the sequence has fewer tokens than new ones
   int e0;     // first entry of kv_indices
   int total;  // tokens with the new ones
 };
@@ -55,12 +56,13 @@ __device__ __forceinline__ Seq load_seq(const AttnParams &p, int i, bool report)
     total = 0;
   }
   s.total = static_cast<int>(total);
-  s.fresh = fresh > 0 && s.q0 >= 0 ? static_cast<int>(min(fresh, p.num_tokens)) : 0;
-  if (report && s.fresh > 0 && s.q0 + fresh > p.num_tokens) raise_deverr(p.error_word, YL_DEVERR_TOKEN_COUNT);
-  if (p.max_new > 0 && s.fresh > p.max_new) {
-    if (report) raise_deverr(p.error_word, YL_DEVERR_TOKEN_COUNT);
-    s.fresh = 0;
-  }
+  s.first = s.fresh = 0;
+  if (fresh <= 0 || s.q0 < 0) return s;
+  s.first = static_cast<int>(total - fresh);  // (fresh is below 2^31, as q0 is not negative)
+  const bool whole = s.q0 + fresh <= p.num_tokens, fits = p.max_new == 0 || fresh <= p.max_new;
+  if (report && !(whole && fits)) raise_deverr(p.error_word, YL_DEVERR_TOKEN_COUNT);
+  // rows past the last of q keep those in front of them where they are
+  if (fits) s.fresh = static_cast<int>(whole ? fresh : max(p.num_tokens - s.q0, int64_t(0)));
   return s;
 }
 
@@ -72,16 +74,16 @@ struct Span {
 
 __device__ __forceinline__ Span span_of(const AttnParams &p, const Seq &s, int t0, int t1) {
   Span r;
-  const int p0 = max(s.total - s.fresh + t0, -1);
-  r.end = max(min(s.total - s.fresh + t1, s.total), 0);
-  r.low = p.window > 0 ? min(max(0, p0 + 1 - min(p.window, 1 << 30)), r.end) : 0;
+  const int p0 = max(s.first + t0, -1);
+  r.end = max(min(s.first + t1, s.total), 0);
+  r.low = p.window > 0 ? min(max(0, p0 + 1 - p.window), r.end) : 0;
   r.head = p.window > 0 ? min(p.sinks, r.low) : 0;
   return r;
 }
 
 // Whether the query at position pos sees position j.
 __device__ __forceinline__ bool sees(const AttnParams &p, int pos, int j) {
-  return j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks);
+  return j <= pos && (p.window == 0 || pos - j < p.window || j < p.sinks);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {

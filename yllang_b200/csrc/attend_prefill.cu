@@ -106,7 +106,7 @@ constexpr int kFirst = 1, kLast = 2, kPlans = 4;
 // And on an item.
 struct ItemInfo {
   int tiles;  // 0: there are no more items
-  int q0, fresh, total;
+  int q0, first;  // of its sequence: row of q and o, position
   int head, row0, rows;
 };
 
@@ -168,6 +168,7 @@ class Walker {
         Seq s;
         s.q0 = __shfl_sync(0xffffffffu, seq_.q0, at);
         s.fresh = __shfl_sync(0xffffffffu, seq_.fresh, at);
+        s.first = __shfl_sync(0xffffffffu, seq_.first, at);
         s.e0 = __shfl_sync(0xffffffffu, seq_.e0, at);
         s.total = __shfl_sync(0xffffffffu, seq_.total, at);
         const int64_t units = __shfl_sync(0xffffffffu, units_, at);
@@ -180,8 +181,8 @@ class Walker {
         const int t0 = p_.by_group.div(out.row0);
         const int t1 = p_.by_group.div(min(out.rows, out.row0 + Shape<D>::kRows) - 1) + 1;
         out.span = span_of(p_, s, t0, t1);
-        out.first_pos = s.total - s.fresh + t0;
-        out.last_pos = s.total - s.fresh + t1 - 1;
+        out.first_pos = max(s.first + t0, -1);  // (-1, like all below it, sees nothing)
+        out.last_pos = max(s.first + t1 - 1, -1);
         constexpr int KT = Shape<D>::kKT;
         out.head_tiles = (out.span.head + KT - 1) / KT;
         out.tiles = max(1, out.head_tiles + (out.span.end - out.span.low + KT - 1) / KT);
@@ -522,7 +523,7 @@ __device__ __forceinline__ void plan_tiles(const AttnParams &p, Shared *sh) {
     const bool more = walker.seek(n, it);
     if (!warp_wait(p, &sh->item_empty[items & 1], (items >> 1 & 1) ^ 1)) return;
     if (lane == 0) {
-      sh->item[items & 1] = ItemInfo{more ? it.tiles : 0, it.seq.q0, it.seq.fresh, it.seq.total, it.head, it.row0, it.rows};
+      sh->item[items & 1] = ItemInfo{more ? it.tiles : 0, it.seq.q0, it.seq.first, it.head, it.row0, it.rows};
       mbar_arrive(&sh->item_full[items & 1]);
       if (more) n = static_cast<int64_t>(gridDim.x) + atomicAdd(p.items, 1);
     }
@@ -708,7 +709,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
       used += it.tiles;
       continue;
     }
-    const int pos = it.total - it.fresh + static_cast<int>(p.by_group.div(min(it.row0 + w * 128 + r, it.rows - 1)));
+    const int pos = max(it.first + static_cast<int>(p.by_group.div(min(it.row0 + w * 128 + r, it.rows - 1))), -1);
     // Rows move between global and shared memory in whole: 16-byte chunk
     // `chunk` of rows r0, r0 + STEP, .. is this thread's.
     constexpr int CH = D / 8, STEP = kTileThreads / CH, PER = 128 / STEP;

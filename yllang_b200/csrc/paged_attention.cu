@@ -147,7 +147,7 @@ extern "C" int yl_paged_attention(const yl_paged_attention_args *a, cudaStream_t
   p.heads = a->num_kv_heads;
   p.group = a->num_q_heads / a->num_kv_heads;
   p.page_size = a->page_size;
-  p.window = a->window;
+  p.window = std::min(a->window, 1 << 30);  // (no sequence is longer; positions minus it stay in 32 bits)
   p.sinks = a->sinks;
   p.max_new = a->max_new_len;
   p.by_page = FastDiv(static_cast<uint32_t>(a->page_size));
