@@ -117,3 +117,27 @@ def test_rows_that_are_there_keep_their_positions(cuda, kv, new, have, window):
     assert int(err.item()) == yl.DEVERR_TOKEN_COUNT
     want, spread, reach = attention_reference(q, kx, vx, [prior], [new], pages, window, 2)
     _check(got, want[:have], spread[:have], reach[:have], torch.float16, kv, D)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kv", ["e4m3", "16"])
+def test_items_of_one_row_tile_behind_items_of_two(cuda, D, kv):
+    """Sequences of 296 query rows (one item of one row tile, one of two, per
+    head, several items to an SM) whose last value is no number: the rows in
+    front of it give bit for bit what they give where it is 0, each time."""
+    H, ps, B, new = 3, 16, 60, 296
+    P = B * 20
+    idx, pages = make_index([7] * B, [new] * B, ps, P, 1)
+    (k, v, ks, vs), _ = _pool(P, ps, H, D, torch.bfloat16, kv, cuda, 2)
+    q = torch.randn(B * new, H, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda)
+    last = torch.tensor([mine[(7 + new - 1) // ps] for mine in pages], device=cuda), (7 + new - 1) % ps
+    call = lambda: yl.paged_attention(q, k, v, idx, k_scale=ks, v_scale=vs)  # noqa: E731
+    place, zero, nan = (v.view(torch.uint8), 0, 0x7F) if kv == "e4m3" else (v, 0.0, float("nan"))
+    place[last] = zero
+    want = call().view(B, new, H, D)
+    assert bool(torch.isfinite(want).all())
+    place[last] = nan
+    for _ in range(8):
+        got = call().view(B, new, H, D)
+        assert torch.equal(got[:, :-1], want[:, :-1])
+        assert bool(torch.isnan(got[:, -1]).all())

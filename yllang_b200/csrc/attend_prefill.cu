@@ -114,6 +114,7 @@ struct Shared {
   uint64_t k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages];
   uint64_t item_full[2], item_empty[2], plan_full[kPlans], plan_empty[kPlans];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t described[2];  // a row tile has read the last of an item's descriptions
   uint64_t drained;
   uint32_t tmem;
   float top[2][2][kLoadWarps];     // [parity][K, V][loading warp]: largest scales
@@ -603,6 +604,13 @@ __device__ __forceinline__ void issue_products(const AttnParams &p, Shared *sh, 
         tc_fence_after();
         scores(w, tile, w == live - 1);
       }
+      // A row tile that this item lacks may still be at the end of an item before,
+      // whose last tile's description must not be written over: that is done for
+      // the fourth tile behind it, once the keys of the second are used up, by a
+      // product that is behind this wait.  (The row tile's next item is too, so the
+      // barrier is in this phase or just past it.)
+      for (int w = live; w < S::kQTiles && ok; ++w)
+        ok = queries[w] == 0 || warp_wait(p, &sh->described[w], (queries[w] - 1) & 1);
       if (!ok) break;
     }
     const int live = info->live;
@@ -888,6 +896,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams &p, Shared *sh, ui
     if (edge) look_back(used - 1);
     *mine = ghostly ? NAN : l;
     tile_barrier(w, false);
+    if (tid == 0) mbar_arrive(&sh->described[w]);
     l = (ghostly ? NAN : l) + *other;
     const float inv = l == 0.f ? 0.f : value / l;
     // through the shared memory of the queries, which are used up
@@ -944,6 +953,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
       mbar_init(&sh->plan_empty[2 * i], kLoadWarps);
       mbar_init(&sh->plan_empty[2 * i + 1], kLoadWarps);
       mbar_init(&sh->o_full[i], 1);
+      mbar_init(&sh->described[i], 1);
     }
     mbar_init(&sh->drained, 1);
     fence_mbar_init();
