@@ -439,8 +439,12 @@ typedef struct yl_quant_pool {
  * and where the scale has grown, the held tokens take it: code = e4m3(code *
  * old scale / scale).  Powers of two make that exact but for e4m3's subnormals,
  * and cost no precision, since e4m3 carries an exponent of its own.  A held
- * page whose scale is not positive and finite sets YL_DEVERR_SCALE and takes
- * the new tokens' scale, its codes unchanged.
+ * scale that is no power of two (a page that another program filled) stays
+ * while it is large enough; then x / scale is the fp32 product of x and the
+ * rounded 1 / scale, and code * (old scale / scale) a product in fp32, so that
+ * within 2^-22 of a rounding border the code may be the border's other one.  A
+ * held page whose scale is not positive and finite sets YL_DEVERR_SCALE and
+ * takes the new tokens' scale, its codes unchanged.
  *
  * Pages outside [0, num_pages) set YL_DEVERR_PAGE_RANGE, entries past
  * kv_indices_capacity YL_DEVERR_INDICES_CAP, rows past num_tokens

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import yllang_b200 as yl
-from _attnutil import attention_reference, make_index, store_reference
+from _attnutil import attention_reference, e4m3, make_index, page_scale, store_reference
 from test_paged_attention_gpu import _check, _pool
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +141,41 @@ def test_items_of_one_row_tile_behind_items_of_two(cuda, D, kv):
         got = call().view(B, new, H, D)
         assert torch.equal(got[:, :-1], want[:, :-1])
         assert bool(torch.isnan(got[:, -1]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ps,count", [(16, 1), (16, 9), (64, 1), (64, 50), (4, 1), (4, 3)])
+@pytest.mark.parametrize("scale", [7.0, 0.3, 1.0, 15 * 2.0 ** -7, 1e-3])
+def test_store_beside_a_scale_that_is_no_power_of_two(cuda, dtype, ps, count, scale):
+    """A page whose scale another program chose keeps it while it is large
+    enough, and codes are of the product with its fp32 reciprocal: off from x by
+    half a step of e4m3 (2^-4 of the value, 2^-10 below its normal numbers) and
+    the reciprocal's and the product's roundings.  Louder tokens bring the power
+    of two that they need, and the held codes are multiplied by the quotient."""
+    H, D, P, held = 3, 64, 2, 1
+    idx, pages = make_index([held], [count], ps, P, 1)
+    page = pages[0][0]
+    g = torch.Generator().manual_seed(count)
+    s = torch.tensor(scale)
+    for grow in (False, True):
+        pool = yl.quant_kv_pool(P, ps, H, D, device=cuda)
+        for t in (pool.k, pool.v):
+            t.view(torch.uint8).copy_(torch.randint(0, 127, t.shape, generator=g, dtype=torch.uint8))
+        pool.k_scale.fill_(scale)
+        pool.v_scale.fill_(scale)
+        before = pool.k[page, :held].cpu().float()
+        x = torch.randint(-255, 256, (count, H, D), generator=g).float()
+        x[..., :4] = torch.tensor([175.0, -203.0, 119.0, 77.0])  # borders of a scale of 7
+        x = (x * (s / 7)).to(dtype)
+        if grow:
+            x[0, :, 5] = 1000 * s
+        yl.store_kv_cache_quant(x.to(cuda), x.to(cuda), pool, idx)
+        after = page_scale(float(x[0, 0].double().abs().max())) if grow else s
+        after = torch.as_tensor(after, dtype=torch.float32)
+        assert bool((pool.k_scale[page] == after).all())
+        codes = pool.k[page].cpu()
+        assert torch.equal(codes[held:held + count].double(), e4m3((x.float() * (1 / after)).double()))
+        off = (codes[held:held + count].double() * after.double() - x.double()).abs()
+        assert bool((off <= x.double().abs() * (2.0 ** -4 + 2.0 ** -23) + 2.0 ** -10 * after.double()).all())
+        want = e4m3((before * (s / after)).double()) if grow else before.double()
+        assert torch.equal(codes[:held].double(), want)
