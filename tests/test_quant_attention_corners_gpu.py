@@ -179,3 +179,22 @@ def test_store_beside_a_scale_that_is_no_power_of_two(cuda, dtype, ps, count, sc
         assert bool((off <= x.double().abs() * (2.0 ** -4 + 2.0 ** -23) + 2.0 ** -10 * after.double()).all())
         want = e4m3((before * (s / after)).double()) if grow else before.double()
         assert torch.equal(codes[:held].double(), want)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("prior,new", [(31, 2), (26, 12), (3, 40)])
+def test_scales_of_unseen_pages_do_not_reach_a_query(cuda, which, bad, prior, new):
+    """The last page's scale is no finite number: the queries in front of the
+    page give what they give without it, the others no number."""
+    H, G, D, ps, P = 2, 2, 128, 16, 10
+    idx, pages = make_index([prior], [new], ps, P, 1)
+    (k, v, ks, vs), (kx, vx) = _pool(P, ps, H, D, torch.bfloat16, "e4m3", cuda, 2)
+    q = torch.randn(new, H * G, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    (ks if which == "k" else vs)[pages[0][2]] = bad
+    got = yl.paged_attention(q.to(cuda), k, v, idx, k_scale=ks, v_scale=vs)
+    want, spread, reach = attention_reference(q, kx, vx, [prior], [new], pages)
+    before = 2 * ps - prior
+    _check(got, want, spread, reach, torch.bfloat16, "e4m3", D, rows=slice(0, before))
+    if which == "v" or bad != bad:
+        assert not bool(torch.isfinite(got[before:]).all(-1).any())

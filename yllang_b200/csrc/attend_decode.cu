@@ -593,6 +593,16 @@ __device__ __forceinline__ void compute_units(const AttnParams &p, const Place &
     }
     if (flags & kRagged) {
       ghosts = clean_values<D, Q8, BF, L::kTokens>(sv, t0);
+      if (Q8) {  // a V scale that is no number counts like such values
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (!is_number(vs[t][k])) {
+              vs[t][k] = 0.f;
+              ghosts |= 1u << (16 * t + r + 8 * k);
+            }
+      }
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll

@@ -86,6 +86,9 @@ __device__ __forceinline__ bool sees(const AttnParams &p, int pos, int j) {
   return j <= pos && (p.window == 0 || pos - j < p.window || j < p.sinks);
 }
 
+// Neither an infinity nor NaN.
+__device__ __forceinline__ bool is_number(float x) { return fabsf(x) < __int_as_float(0x7f800000); }
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }

@@ -355,7 +355,9 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
     const Plan &t0 = plan(used);
 
     if (Q8) {
-      float ktop = ks0, vtop = vs0;
+      // (a scale that is no number is left out here and becomes NaN below, which
+      // reaches the rows that see its token as such values do)
+      float ktop = is_number(ks0) ? ks0 : 0.f, vtop = is_number(vs0) ? vs0 : 0.f;
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) {
         ktop = fmaxf(ktop, __shfl_xor_sync(0xffffffffu, ktop, d));
@@ -383,7 +385,8 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
         value = vtop;
       }
       if (tid < KT) {
-        const float rk = ks0 / key, rv = value > 0.f ? vs0 / value : 0.f;
+        const float rk = is_number(ks0) ? ks0 / key : NAN;
+        const float rv = !is_number(vs0) ? NAN : value > 0.f ? vs0 / value : 0.f;
         sh->ratio[par][0][tid] = Fp16::pack(rk, rk);
         sh->ratio[par][1][tid] = Fp16::pack(rv, rv);
       }
