@@ -355,14 +355,13 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
     const Plan &t0 = plan(used);
 
     if (Q8) {
-      // (a scale that is no number is left out here and becomes NaN below, which
-      // reaches the rows that see its token as such values do)
-      float ktop = is_number(ks0) ? ks0 : 0.f, vtop = is_number(vs0) ? vs0 : 0.f;
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) {
-        ktop = fmaxf(ktop, __shfl_xor_sync(0xffffffffu, ktop, d));
-        vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
-      }
+      // (positive numbers are ordered like their bits; a scale that is no number is
+      // left out here and reaches the rows that see its token with its codes)
+      auto largest = [](float s) {
+        const uint32_t b = __float_as_uint(s);
+        return __uint_as_float(__reduce_max_sync(0xffffffffu, b < 0x7f800000u ? b : 0u));
+      };
+      const float ktop = largest(ks0), vtop = largest(vs0);
       if (lane == 0) {
         sh->top[par][0][warp] = ktop;
         sh->top[par][1][warp] = vtop;
@@ -385,8 +384,7 @@ __device__ __forceinline__ void load_tiles(const AttnParams &p, Shared *sh, uint
         value = vtop;
       }
       if (tid < KT) {
-        const float rk = is_number(ks0) ? ks0 / key : NAN;
-        const float rv = !is_number(vs0) ? NAN : value > 0.f ? vs0 / value : 0.f;
+        const float rk = ks0 / key, rv = vs0 / (value > 0.f ? value : 1.f);
         sh->ratio[par][0][tid] = Fp16::pack(rk, rk);
         sh->ratio[par][1][tid] = Fp16::pack(rv, rv);
       }
