@@ -515,9 +515,22 @@ YL_API int yl_kv_quant_load(const yl_quant_load_args *args, cudaStream_t stream)
  * sequence sees are not read, and their entries of kv_indices may hold
  * anything (a window's pages can be given back while their entries stay).
  * Where a query sees a V row that holds an infinity or NaN, any element of
- * its result may be NaN.  Any number of new tokens per sequence, none
- * included, and any page size.  Rows of o in front of qo_indptr[0] and behind
+ * its result may be NaN; so it may where a scale that it sees is no number.
+ * Sums are divided by the sum of weights at the end, so V elements of 2^80 and
+ * more may overflow.  Any number of new tokens per sequence, none included, and
+ * any page size.  Rows of o in front of qo_indptr[0] and behind
  * qo_indptr[B] stay as they were.  o must not overlap q or the pool.
+ *
+ * The products of an 8-bit pool are of fp16 operands, which hold e4m3 codes and
+ * powers of two exactly.  Scales may be any positive numbers, within these
+ * limits (KS, VS: the largest scales of K and of V among the pages that the new
+ * tokens of a sequence see, for a KV head).  A scale that is no power of two
+ * rounds its page's elements by up to 2^-10 of each.  Under 2^-15 KS (VS) an
+ * element is also off by up to 2^-25 KS (VS), so that a page under 2^-24 VS may
+ * add nothing even where its tokens have all of the weight.  A token's weight,
+ * beside its relative rounding to fp16, is off by up to 2^-28 of the largest, and
+ * its weight times V scale by up to 2^-36 VS.  (Pages that the store filled with
+ * values within 2^15 of one another's meet none of the first two.)
  *
  * A seen page outside [0, num_pages) sets YL_DEVERR_PAGE_RANGE and counts as
  * not seen, entries past kv_indices_capacity YL_DEVERR_INDICES_CAP likewise;

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import yllang_b200 as yl
-from _attnutil import attention_reference, e4m3, make_index, page_scale, store_reference
+from _attnutil import attention_bound, attention_reference, e4m3, make_index, page_scale, store_reference
 from test_paged_attention_gpu import _check, _pool
 
 pytestmark = pytest.mark.gpu
@@ -198,3 +198,120 @@ def test_scales_of_unseen_pages_do_not_reach_a_query(cuda, which, bad, prior, ne
     _check(got, want, spread, reach, torch.bfloat16, "e4m3", D, rows=slice(0, before))
     if which == "v" or bad != bad:
         assert not bool(torch.isfinite(got[before:]).all(-1).any())
+
+
+def _wide_bound(want, spread, reach, dtype, D, scores, values, sums):
+    """attention_bound where scores are off by `scores` more, values by a part
+    of `values`, and the result by `sums`."""
+    grown = torch.exp(2 * scores) - 1  # of a weight over the sum of weights
+    return attention_bound(want, spread * (1 + grown), reach, dtype, torch.float16, D) + spread * (grown + values) + sums
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("ps", [5, 16, 128])
+@pytest.mark.parametrize("window", [0, 60])
+def test_scales_that_are_no_powers_of_two(cuda, dtype, D, ps, window):
+    """Any fp32 scales, decode and prefill: the elements of a page are off by
+    2^-10 at most (prefill rounds scale and product to fp16, half a step of
+    2^-11 each), so scores by 2^-10 of the sum of |q| |k|."""
+    H, G = 2, 4
+    prior, new = [0, 37, 100], [60, 20, 1]
+    P = sum(-(-(a + b) // ps) for a, b in zip(prior, new)) + 2
+    idx, pages = make_index(prior, new, ps, P, 1)
+    (k, v, ks, vs), (kx, vx) = _pool(P, ps, H, D, dtype, "e4m3", cuda, 2)
+    g = torch.Generator().manual_seed(4)
+    for s, x in ((ks, kx), (vs, vx)):
+        other = s.cpu() * (1 + torch.rand(s.shape, generator=g))
+        x.mul_((other.double() / s.double().cpu())[:, None, :, None])
+        s.copy_(other)
+    q = (torch.randn(sum(new), H * G, D, generator=g) / 2).to(dtype)
+    got = yl.paged_attention(q.to(cuda), k, v, idx, k_scale=ks, v_scale=vs, window=window, sinks=3).cpu().double()
+    want, spread, reach = attention_reference(q, kx, vx, prior, new, pages, window, 3)
+    bound = _wide_bound(want, spread, reach, dtype, D, 2.0 ** -10 * reach, 2.0 ** -10, 0)
+    assert float(((got - want).abs() / bound).max()) <= 1
+    rows = slice(sum(new) - 1, None)  # decode: scales stay in fp32, weights are rounded once
+    bound = attention_bound(want, spread, reach, dtype, torch.float16, D)
+    assert float(((got - want).abs() / bound)[rows].max()) <= 1
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("place", [0, 1, 3])
+@pytest.mark.parametrize("far", [0, 8, 15, 16, 20, 24, 40])
+def test_a_page_of_small_values_with_all_the_weight(cuda, new, place, far):
+    """One page's V scale lies 2^far under the others', and all of the weight on
+    its tokens: down to 2^-15 the result is as exact as ever, and below off by
+    2^-25 of the largest scale.  The page may be the first, the last or between."""
+    H, G, D, ps, P, total = 2, 2, 64, 64, 6, 256
+    idx, pages = make_index([0], [total], ps, P, 1)
+    idx = idx._replace(qo_indptr=torch.tensor([0, new], dtype=torch.int32, device=cuda))
+    (k, v, ks, vs), (_, vx) = _pool(P, ps, H, D, torch.float16, "e4m3", cuda, 2)
+    codes = vx / vs.double().cpu()[:, None, :, None]
+    page = pages[0][place]
+    vs.fill_(1.0)
+    vs[page] = 2.0 ** -far
+    ks.fill_(2.0 ** -3)
+    kx = torch.full((P, ps, H, D), -1.0, dtype=torch.float64)  # scores of about 20, the page's, and -20
+    kx[page] = 1.0 + torch.arange(ps)[:, None, None].double() % 3 / 8
+    k.view(torch.uint8).copy_((kx * 8).to(torch.float8_e4m3fn).view(torch.uint8).to(cuda))
+    vx = codes * vs.double().cpu()[:, None, :, None]
+    q = 2.5 + torch.rand(new, H * G, D, generator=torch.Generator().manual_seed(3)) / 4
+    q = q.to(torch.float16)
+    got = yl.paged_attention(q.to(cuda), k, v, idx, k_scale=ks, v_scale=vs).double().cpu()
+    want, spread, reach = attention_reference(q, kx, vx, [total - new], [new], pages)
+    seen = torch.arange(total - new, total) >= place * ps + ps - 1  # queries that see all of the page
+    size = codes.abs()[pages[0]].sum((0, 1)).repeat_interleave(G, 0)  # sum of |codes| of the sequence's tokens
+    small = codes.abs()[page].sum(0).repeat_interleave(G, 0)
+    # (the others' weights are e^-40 and less: lost or not, 2^-36 of their codes bounds them)
+    sums = 2.0 ** -36 * size + 2.0 ** (-28 - far) * small + (2.0 ** -25 if far > 15 else 0)
+    sums = sums + 2.0 ** -25  # half of fp16's smallest step, of the result
+    bound = _wide_bound(want, spread, reach, torch.float16, D, 0 * reach, 0, sums)
+    assert bool(seen.any())
+    assert float(((got - want).abs() / bound)[seen].max()) <= 1
+    if far <= 8:  # and the bound is one that a lost page would not pass
+        assert float((want.abs() / bound)[seen].median()) > 16
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("far", [0, 15, 18, 22])
+def test_a_page_of_small_keys_with_all_the_weight(cuda, new, far):
+    """A page whose K scale lies 2^far above the others' and whose scores lie far
+    below theirs: the others' keep their precision down to 2^-15, and elements
+    are off by 2^-25 of the largest scale below."""
+    H, G, D, ps, P, total = 2, 2, 64, 16, 8, 64
+    idx, pages = make_index([0], [total], ps, P, 1)
+    idx = idx._replace(qo_indptr=torch.tensor([0, new], dtype=torch.int32, device=cuda))
+    (k, v, ks, vs), (kx, vx) = _pool(P, ps, H, D, torch.bfloat16, "e4m3", cuda, 2)
+    page = pages[0][0]
+    kx = kx / ks.double().cpu()[:, None, :, None]
+    kx[page] = -kx[page].abs().clamp(min=16)
+    k.view(torch.uint8).copy_(kx.to(torch.float8_e4m3fn).view(torch.uint8).to(cuda))
+    ks.fill_(2.0 ** -8)
+    ks[page] = 2.0 ** (far - 8)
+    kx = kx * ks.double().cpu()[:, None, :, None]
+    q = (1 + torch.rand(new, H * G, D, generator=torch.Generator().manual_seed(3))).to(torch.bfloat16)
+    got = yl.paged_attention(q.to(cuda), k, v, idx, k_scale=ks, v_scale=vs).double().cpu()
+    want, spread, _ = attention_reference(q, kx, vx, [total - new], [new], pages)
+    if far:
+        kx[page] = 0  # scores of -2^15 and less, whose own error does not matter
+    _, _, reach = attention_reference(q, kx, vx, [total - new], [new], pages)
+    scores = 2.0 ** -25 * float(ks.max()) * q.double().abs().sum(-1, keepdim=True) * D ** -0.5 if far > 15 else 0 * reach
+    bound = _wide_bound(want, spread, reach, torch.bfloat16, D, scores, 0, 0)
+    assert float(((got - want).abs() / bound).max()) <= 1
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("kv", ["e4m3", "16"])
+def test_values_near_the_largest_allowed(cuda, new, kv):
+    """V elements just under 2^80 come through."""
+    H, G, D, ps, P = 2, 2, 64, 16, 8
+    idx, pages = make_index([60], [new], ps, P, 1)
+    (k, v, ks, vs), (kx, vx) = _pool(P, ps, H, D, torch.bfloat16, kv, cuda, 2)
+    up = 2.0 ** 70
+    (v if kv == "16" else vs).mul_(up)
+    vx = vx * up
+    assert float(vx.abs().max()) < 2.0 ** 80
+    q = torch.randn(new, H * G, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    got = yl.paged_attention(q.to(cuda), k, v, idx, k_scale=ks, v_scale=vs)
+    want, spread, reach = attention_reference(q, kx, vx, [60], [new], pages)
+    _check(got, want, spread, reach, torch.bfloat16, kv, D)

@@ -35,7 +35,8 @@
 //   interleaved by byte permutes before conversion.  K's scale multiplies the
 //   scores; V's scale, relative to the largest seen so far, multiplies the
 //   weights before they are rounded.  Weights are kept times 2^11, so the largest
-//   is at most 2^15 and fp16's smallest numbers lie 2^-35 below the reference.
+//   is at most 2^15, and times V's scale their smallest steps are 2^-35 of the
+//   largest weight times the largest scale.
 // * All sums, maxima and accumulators are fp32; weights are rounded once, to
 //   fp16 (8-bit and fp16 pools) or bf16 (bf16 pools), as the matrix
 //   instructions take them.

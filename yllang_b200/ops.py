@@ -540,6 +540,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     16-bit pool), or float8_e4m3fn with k_scale, v_scale fp32 [P, H] (a
     QuantKVPool layer).  Hq is a multiple of H; D is 64, 128 or 256.
 
+    Scales of an 8-bit pool may be any positive numbers; powers of two within
+    2^15 of the largest that a sequence sees, which the store writes for values
+    of one order, lose nothing (the limits of others: yl_paged_attention).
+
     window > 0: a query at position p sees positions above p - window, and the
     first `sinks` positions; pages that no new token sees are not read.
     sm_scale: 1 / sqrt(D) by default.  max_new_len: an upper bound of the new
