@@ -4,11 +4,12 @@
 // it: 2 * visible tokens * head_dim * item bytes per KV head.  What the design
 // is for is keeping every SM's loads in flight to the end:
 //
-// * The batch's work is one line of units, a unit being a tile of 64 visible
-//   tokens of one (sequence, KV head, 16 query rows); the query rows of a unit
-//   are the new tokens times the heads of the group.  Each CTA takes an equal
-//   run of that line, whatever the lengths of the sequences; each finds its
-//   place by scanning the batch itself (a few KB), so a call needs no plan.
+// * The batch's work is one line of units, a unit being a tile of visible tokens
+//   (128 where a head's row is 128 bytes or less, else 64) of one (sequence, KV
+//   head, 8 or 16 query rows); the query rows of a unit are the new tokens times
+//   the heads of the group.  Each CTA takes an equal run of that line, whatever
+//   the lengths of the sequences; each finds its place by scanning the batch
+//   itself (a few KB), so a call needs no plan.
 //   A (sequence, head) whose units fall in several CTAs leaves its parts in the
 //   workspace, and a second kernel joins them, in a fixed order.
 // * Four warps of a CTA only issue loads, a quarter of a unit's tokens each: they
@@ -28,15 +29,16 @@
 //   from the first product's result to the second's operand by a transposing
 //   register move.
 // * An 8-bit pool is multiplied in fp16: every e4m3 value is exact there.  bf16
-//   queries are first brought into fp16's range by a power of two per row,
-//   exact for all elements within 2^-24 of the row's largest.  The contraction
-//   order of k.q is free, so a lane takes 4 neighbouring codes as its part of a
-//   k-step and K needs no transposition; the codes of two tokens of V are
-//   interleaved by byte permutes before conversion.  K's scale multiplies the
-//   scores; V's scale, relative to the largest seen so far, multiplies the
-//   weights before they are rounded.  Weights are kept times 2^11, so the largest
-//   is at most 2^15, and times V's scale their smallest steps are 2^-35 of the
-//   largest weight times the largest scale.
+//   queries are first brought into fp16's range by a power of two per row, exact
+//   for all elements within 2^-17 of the row's largest (8 bits above fp16's
+//   smallest step) and off by up to 2^-25 of it below.  The contraction order of
+//   k.q is free, so a lane takes 4 neighbouring codes as its part of a k-step and
+//   K needs no transposition; the codes of two tokens of V are interleaved by byte
+//   permutes before conversion.  K's scale multiplies the scores; V's scale,
+//   relative to the largest seen so far, multiplies the weights before they are
+//   rounded.  Weights are kept times 2^11, so the largest is at most 2^15, and
+//   times V's scale their smallest steps are 2^-35 of the largest weight times the
+//   largest scale.
 // * All sums, maxima and accumulators are fp32; weights are rounded once, to
 //   fp16 (8-bit and fp16 pools) or bf16 (bf16 pools), as the matrix
 //   instructions take them.

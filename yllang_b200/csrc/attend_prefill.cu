@@ -11,13 +11,13 @@
 //   and leave them 16-bit and swizzled in a ring of two stages.  16-bit pools
 //   are copied asynchronously; the codes of an 8-bit pool are converted on the
 //   way to fp16, which holds every e4m3 value (K's wait for it in shared memory
-//   while the tile before is converted, V's in registers).  K's scales, relative to the
-//   largest of the tile, are multiplied in: exact for powers of two down to 2^-15,
-//   two roundings to fp16 for others (factors per column in the softmax instead
-//   cost all 8-bit tiles 11 %, for the registers).  The tile's largest goes to the
-//   scores as one factor.  V's are multiplied in relative to
-//   a reference that changes only when a tile's largest passes 64 times it, when
-//   the accumulators are rescaled.
+//   while the tile before is converted, V's in registers).  K's scales, relative
+//   to the largest of the tile, are multiplied in: exact for powers of two down to
+//   2^-15, two roundings to fp16 for others (factors per column in the softmax
+//   instead cost all 8-bit tiles 11 %, for the registers).  The tile's largest goes
+//   to the scores as one factor.  V's are multiplied in relative to a reference
+//   that changes only when a tile's largest passes 64 times it, when the
+//   accumulators are rescaled.
 // * Warp 24 issues the products: S = Q K^T per 128 rows (both operands in shared
 //   memory), O += P V (P in tensor memory).  The two row tiles alternate, so
 //   that one's products run while the other's softmax does.  Warp 25 plans: it

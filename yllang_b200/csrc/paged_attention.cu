@@ -16,9 +16,9 @@ namespace {
 // sequence is the decode kernel's.  It reads the keys once for each 16 rows, in
 // parts over all SMs; the prefill kernel once for 256, by one SM.  32 sequences
 // of up to 8k tokens, 8-bit, 8 KV heads of 128: 32 rows 152 us against 324, 64
-// rows 286 against 332, 128 rows 556 against 331.  (One sequence alone still
-// gains at 128 rows, 35 us against 119; the rule does not look at the batch,
-// whose lengths the host does not know.)
+// rows 286 against 332, 128 rows 556 against 331.  The rule looks at a sequence's
+// rows only: one sequence alone, whose items are fewer than the SMs, loses by it
+// (at 128 rows 119 us, 35 in the decode kernel).
 constexpr int kDecodeRows = 64;
 
 // Most query rows per KV head that a sequence of the call can have.
