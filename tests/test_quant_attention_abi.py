@@ -3,6 +3,7 @@ points, without a GPU: every argument error comes back as a status before any
 launch, empty calls are no-ops, and the Python and C++ front ends refuse tensors
 of the wrong kind."""
 import ctypes
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -200,6 +201,19 @@ def test_front_ends_refuse_host_tensors_and_wrong_kinds():
         yl.paged_attention(q[0], q, q, _index())
     with pytest.raises(yl.PanicError, match="CUDA"):
         yl.paged_attention_workspace(q, q, q, _index())
+
+
+def test_front_ends_refuse_a_stream_of_another_device():
+    """Such a call would otherwise run on the current stream of the tensors' device."""
+    stream = SimpleNamespace(device=torch.device("cuda", 1))
+    pool = yl.quant_kv_pool(4, 16, 2, 64, device="cpu")
+    rows = torch.zeros(3, 128, dtype=torch.bfloat16)
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    for call in (lambda: yl.store_kv_cache_quant(rows, rows, pool, _index(), stream=stream),
+                 lambda: yl.load_kv_cache_quant(pool, torch.zeros(3, dtype=torch.int64), stream=stream),
+                 lambda: yl.paged_attention(q, q, q, _index(), stream=stream)):
+        with pytest.raises(yl.PanicError, match="stream is on cuda:1"):
+            call()
 
 
 def test_quant_pool_layout():
