@@ -484,7 +484,8 @@ def _run(call, what: str, device: torch.device, stream: torch.cuda.Stream | None
     """One call of the front end on `stream`, its refusals as this module's PanicError."""
     C = _front_end()
     # (entering another device's stream would leave this device's current one in its place)
-    _check(stream is None or stream.device == device, f"{what}: stream is on {stream and stream.device}, tensors on {device}")
+    if stream is not None and stream.device != device:
+        raise PanicError(f"{what}: stream is on {stream.device}, tensors on {device}")
     try:
         if stream is None and not CHECK_DEVICE_ERRORS:
             return call(*args, error_word)
