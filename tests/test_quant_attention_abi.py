@@ -154,6 +154,19 @@ def test_paged_attention_rejects_bad_arguments_on_host(kw, status):
     assert _abi.last_error().startswith("yl_paged_attention")
 
 
+@pytest.mark.parametrize("call,make,names", [
+    (_abi.kv_quant_store_raw, _store, ["kv_indptr", "kv_indices", "kv_last_page_len", "qo_indptr", "error_word"]),
+    (_abi.kv_quant_load_raw, _load, ["error_word"]),
+    (_abi.paged_attention_raw, _attend, ["kv_indptr", "kv_indices", "kv_last_page_len", "qo_indptr", "k_scale", "v_scale",
+                                         "error_word"]),
+], ids=["store", "load", "attention"])
+def test_words_off_their_alignment_are_refused(call, make, names):
+    """A kernel would fault on them."""
+    for name in names:
+        assert call(make(**{name: 0x9002}), None) == _abi.YL_ERR_ALIGNMENT, name
+        assert "4-byte aligned" in _abi.last_error()
+
+
 def test_empty_calls_are_noops_without_device():
     L = yl.lib()
     assert _abi.kv_quant_store_raw(_store(num_tokens=0, k=0), None) == _abi.YL_OK

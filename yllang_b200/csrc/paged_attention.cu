@@ -77,6 +77,13 @@ int check_attention(const yl_paged_attention_args *a, bool pointers) {
   if (bits & 15u)
     return fail(YL_ERR_ALIGNMENT, "yl_paged_attention: pointers and strides of q, o and the pool must be multiples of "
                                   "16 bytes");
+  const uintptr_t words =
+      reinterpret_cast<uintptr_t>(a->kv_indptr) | reinterpret_cast<uintptr_t>(a->kv_indices) |
+      reinterpret_cast<uintptr_t>(a->kv_last_page_len) | reinterpret_cast<uintptr_t>(a->qo_indptr) |
+      reinterpret_cast<uintptr_t>(a->error_word) |
+      (a->kv_dtype == YL_KV_E4M3 ? reinterpret_cast<uintptr_t>(a->k_scale) | reinterpret_cast<uintptr_t>(a->v_scale) : 0);
+  if (words & 3u)
+    return fail(YL_ERR_ALIGNMENT, "yl_paged_attention: page arrays, scales and error_word must be 4-byte aligned");
   return YL_OK;
 }
 

@@ -643,6 +643,10 @@ extern "C" int yl_kv_quant_store(const yl_quant_store_args *a, cudaStream_t stre
   if (!a->k || !a->v || !a->kv_indptr || !a->kv_last_page_len || !a->qo_indptr ||
       (!a->kv_indices && a->kv_indices_capacity > 0))
     return fail(YL_ERR_NULL_ARG, "yl_kv_quant_store: k, v and the page arrays must be non-NULL");
+  if ((reinterpret_cast<uintptr_t>(a->kv_indptr) | reinterpret_cast<uintptr_t>(a->kv_indices) |
+       reinterpret_cast<uintptr_t>(a->kv_last_page_len) | reinterpret_cast<uintptr_t>(a->qo_indptr) |
+       reinterpret_cast<uintptr_t>(a->error_word)) & 3u)
+    return fail(YL_ERR_ALIGNMENT, "yl_kv_quant_store: page arrays and error_word must be 4-byte aligned");
   rc = check_rows(a->k, a->v, a->k_row_stride, a->v_row_stride, a->k_layer_stride, a->v_layer_stride, a->pool, who);
   if (rc != YL_OK) return rc;
   if (a->num_tokens >= (1ll << 31))
@@ -714,6 +718,8 @@ extern "C" int yl_kv_quant_load(const yl_quant_load_args *a, cudaStream_t stream
   const uintptr_t ib = a->slot_is_int64 ? 8 : 4;
   if (reinterpret_cast<uintptr_t>(a->slots) & (ib - 1))
     return fail(YL_ERR_ALIGNMENT, "yl_kv_quant_load: slots pointer is not %lld-byte aligned", (long long)ib);
+  if (reinterpret_cast<uintptr_t>(a->error_word) & 3u)
+    return fail(YL_ERR_ALIGNMENT, "yl_kv_quant_load: error_word must be 4-byte aligned");
   const int64_t planes = 2ll * a->pool.num_layers;
   if (a->num_tokens >= (1ll << 31) / planes / a->pool.num_heads)
     return fail(YL_ERR_UNSUPPORTED, "yl_kv_quant_load: num_tokens=%lld times layers and heads passes 2^31",
