@@ -451,9 +451,9 @@ typedef struct yl_quant_pool {
  * YL_DEVERR_TOKEN_COUNT, more new tokens than the sequence's pages hold
  * YL_DEVERR_ROW_OVERFLOW; each skips those rows.  Rows in front of qo_indptr[0]
  * and behind qo_indptr[B] have no effect, so a slice of a batch's page arrays is
- * a batch over the same rows.  A page that two sequences of one call write is
- * outside the contract.  Row pointers and strides of k and v are multiples of 16
- * bytes, codes of 8.
+ * a batch over the same rows.  A page that one call writes twice, for two
+ * sequences or at two places of one, is outside the contract.  Row pointers and
+ * strides of k and v are multiples of 16 bytes, codes of 8.
  */
 typedef struct yl_quant_store_args {
   yl_quant_pool pool;

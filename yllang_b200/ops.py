@@ -510,7 +510,7 @@ def store_kv_cache_quant(k: torch.Tensor, v: torch.Tensor, pool: QuantKVPool, in
     have no effect, so the arrays may be a slice of a batch's).  Each page
     and head has one power-of-two scale; where new tokens need a larger one,
     the page's earlier tokens take it too (see yl_kv_quant_store).  Pages that
-    two sequences of one call write are outside the contract.  An infinity is
+    one call writes twice are outside the contract.  An infinity is
     stored as the largest code and NaN as NaN, with DEVERR_NONFINITE set."""
     _run(_front_end().StoreKVCacheQuant, "store_kv_cache_quant", k.device, stream, error_word,
          (k, v, *pool, *index[:4]))
