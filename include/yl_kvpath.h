@@ -452,8 +452,9 @@ typedef struct yl_quant_pool {
  * YL_DEVERR_ROW_OVERFLOW; each skips those rows.  Rows in front of qo_indptr[0]
  * and behind qo_indptr[B] have no effect, so a slice of a batch's page arrays is
  * a batch over the same rows.  A page that one call writes twice, for two
- * sequences or at two places of one, is outside the contract.  Row pointers and
- * strides of k and v are multiples of 16 bytes, codes of 8.
+ * sequences or at two places of one, is outside the contract; layer strides of
+ * the pool are positive.  Row pointers and strides of k and v are multiples of
+ * 16 bytes, codes of 8.
  */
 typedef struct yl_quant_store_args {
   yl_quant_pool pool;

@@ -167,6 +167,21 @@ def test_words_off_their_alignment_are_refused(call, make, names):
         assert "4-byte aligned" in _abi.last_error()
 
 
+@pytest.mark.parametrize("kw", [dict(pool_layer_stride=0), dict(pool_scale_layer_stride=0)])
+def test_layers_that_a_store_writes_lie_apart(kw):
+    """An expanded pool would be written by all layers at once; broadcast rows are read."""
+    apart = dict(pool_num_layers=2, pool_layer_stride=1 << 20, pool_scale_layer_stride=64)
+    assert _abi.kv_quant_store_raw(_store(**{**apart, **kw}), None) == _abi.YL_ERR_BAD_SIZE
+    assert "apart" in _abi.last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(k_layer_stride=0), dict(v_layer_stride=0)])
+def test_layers_that_a_load_writes_lie_apart(kw):
+    apart = dict(pool_num_layers=2, k_layer_stride=1 << 20, v_layer_stride=1 << 20)
+    assert _abi.kv_quant_load_raw(_load(**{**apart, **kw}), None) == _abi.YL_ERR_BAD_SIZE
+    assert "apart" in _abi.last_error()
+
+
 def test_empty_calls_are_noops_without_device():
     L = yl.lib()
     assert _abi.kv_quant_store_raw(_store(num_tokens=0, k=0), None) == _abi.YL_OK

@@ -649,6 +649,8 @@ extern "C" int yl_kv_quant_store(const yl_quant_store_args *a, cudaStream_t stre
     return fail(YL_ERR_ALIGNMENT, "yl_kv_quant_store: page arrays and error_word must be 4-byte aligned");
   rc = check_rows(a->k, a->v, a->k_row_stride, a->v_row_stride, a->k_layer_stride, a->v_layer_stride, a->pool, who);
   if (rc != YL_OK) return rc;
+  if (a->pool.num_layers > 1 && (a->pool.layer_stride < 1 || a->pool.scale_layer_stride < 1))
+    return fail(YL_ERR_BAD_SIZE, "yl_kv_quant_store: the pool's layers must lie apart");
   if (a->num_tokens >= (1ll << 31))
     return fail(YL_ERR_UNSUPPORTED, "yl_kv_quant_store: num_tokens=%lld must be below 2^31", a->num_tokens);
   p.x[0] = static_cast<const char *>(a->k);
@@ -715,6 +717,8 @@ extern "C" int yl_kv_quant_load(const yl_quant_load_args *a, cudaStream_t stream
   rc = check_rows(a->k_out, a->v_out, a->k_row_stride, a->v_row_stride, a->k_layer_stride, a->v_layer_stride, a->pool,
                   who);
   if (rc != YL_OK) return rc;
+  if (a->pool.num_layers > 1 && (a->k_layer_stride < 1 || a->v_layer_stride < 1))
+    return fail(YL_ERR_BAD_SIZE, "yl_kv_quant_load: the layers of k_out and v_out must lie apart");
   const uintptr_t ib = a->slot_is_int64 ? 8 : 4;
   if (reinterpret_cast<uintptr_t>(a->slots) & (ib - 1))
     return fail(YL_ERR_ALIGNMENT, "yl_kv_quant_load: slots pointer is not %lld-byte aligned", (long long)ib);
