@@ -44,12 +44,13 @@
 //   instructions take them.
 //
 // Measured, 256 sequences of 128 to 8k tokens, 8 KV heads of 128: 8-bit pages
-// 338 us, 6.1 TB/s of 6.46 that a plain copy reaches; in a loop of seconds the
-// power limit lowers the clock and it is 375; the loads alone take 313, the
-// arithmetic alone 334 before its last step.  16-bit pages 624 us, 6.6 TB/s;
-// head_dim 256 372 us, 5.9 TB/s; head_dim 64 244 us, 4.2 TB/s, where the softmax
-// of a score costs as much as at 128 and carries half the bytes.  One sequence
-// of 8k tokens takes 13 us: two launches and one chain of loads.
+// 379 us in a loop of seconds, where the power limit lowers the clock, 5.5 TB/s of
+// 6.46 that a plain copy reaches; in a burst 340, 6.1 TB/s; the loads alone take
+// 313, the arithmetic alone 334 before its last step.  16-bit pages 627 us, 6.6
+// TB/s; head_dim 256 660 us, 6.3 TB/s; head_dim 64 252 us, 4.1 TB/s, where the
+// softmax of a score costs as much as at 128 and carries half the bytes.  Pages
+// of one token 566 us: an id, an address and a scale each in the loading warps.
+// One sequence of 8k tokens takes 13 us: two launches and one chain of loads.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -963,7 +964,7 @@ template <typename F>
 auto pick(int dtype, int dim, bool q8, int64_t most_rows, F f) {
   auto rows = [&](auto t, auto d, auto q) {
     // 8 query rows a unit where no sequence has more, else 16 (a second block of
-    // columns for 4 rows costs 256 8-bit sequences 429 us instead of 338; rows in
+    // columns for 4 rows costs 256 8-bit sequences 449 us instead of 340; rows in
     // two units instead of one would read the keys twice)
     if (most_rows <= 8) return f(t, d, q, std::integral_constant<int, 1>{});
     return f(t, d, q, std::integral_constant<int, 2>{});

@@ -36,12 +36,15 @@
 // What bounds it: the products are 4 * 128 * 128 * head_dim flops per row tile
 // and key tile, 2,118 cycles for both row tiles at head_dim 128 when nothing else
 // runs; a tile takes about 3,850 cycles in the steady state of a 16-bit pool (an
-// 8k prompt of 32 heads: 518 us, 1,060 TFLOP/s, 0.65 of the library's measured
-// rate) and 4,900 of an 8-bit one (665 us).  The rest is the chain from a score
+// 8k prompt of 32 heads: 517 us, 1,064 TFLOP/s, 0.65 of the library's measured
+// rate) and 4,900 of an 8-bit one (669 us).  The rest is the chain from a score
 // product through the softmax to the value product, which the two row tiles
 // cover only in part, and for 8-bit pools the conversion.  Masked tiles cost
 // about 1,000 cycles more, an item's start and end about 7,000: a window of 1k
-// keys has ten tiles per item, two of them masked, and runs at 0.38.
+// keys has ten tiles per item, two of them masked, and runs at 0.38.  At head_dim
+// 256 there is one row tile an item, so products and softmax take turns (8 prompts
+// of 128 to 4k tokens: 16-bit 1,147 us, 620 TFLOP/s; 8-bit 1,649), and 88 registers
+// are too few for bf16 queries over an 8-bit pool (500 bytes spilled; 178 at 128).
 //
 // Only tiles that some row does not see in full are masked; in those, infinities
 // and NaN of V are zeroed as they are loaded and reported to the rows that see
