@@ -315,3 +315,25 @@ def test_values_near_the_largest_allowed(cuda, new, kv):
     got = yl.paged_attention(q.to(cuda), k, v, idx, k_scale=ks, v_scale=vs)
     want, spread, reach = attention_reference(q, kx, vx, [60], [new], pages)
     _check(got, want, spread, reach, torch.bfloat16, kv, D)
+
+
+@pytest.mark.parametrize("kv,dtype", [("e4m3", torch.bfloat16), ("e4m3", torch.float16), ("16", torch.bfloat16)])
+@pytest.mark.parametrize("window", [0, 700])
+def test_a_mixed_batch_repeats_itself_bit_for_bit(cuda, kv, dtype, window):
+    """Prompts, chunks and decode steps in one call, with work for every SM: the
+    joins' order and the items' way to the SMs do not show in the results."""
+    H, G, D, ps = 8, 4, 128, 16
+    prior = [0, 3000, 511, 4095, 0, 77] + [37 * i % 4000 for i in range(60)]
+    new = [1500, 512, 100, 17, 1, 300] + [1] * 60
+    P = sum(-(-(a + b) // ps) for a, b in zip(prior, new)) + 1
+    idx, _ = make_index(prior, new, ps, P, 1)
+    (k, v, ks, vs), _ = _pool(P, ps, H, D, dtype, kv, cuda, 2)
+    q = torch.randn(sum(new), H * G, D, generator=torch.Generator().manual_seed(3)).to(dtype).to(cuda)
+    other = torch.empty(1 << 26, dtype=torch.uint8, device=cuda)
+    first = None
+    for i in range(12):
+        out = torch.full_like(q, float("nan"))
+        yl.paged_attention(q, k, v, idx, k_scale=ks, v_scale=vs, window=window, sinks=4, out=out)
+        other.fill_(i)  # (something else in the caches and on the SMs)
+        first = out if first is None else first
+        assert bool(torch.isfinite(out).all()) and torch.equal(out, first)
