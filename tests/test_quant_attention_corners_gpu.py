@@ -101,6 +101,23 @@ def test_store_reports_every_missing_row(cuda, batch, ps):
         assert (int(err.item()), written) == (yl.DEVERR_TOKEN_COUNT if rows < n else 0, min(rows, n)), rows
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1], [20, 9, 1], [40, 30, 16]])
+@pytest.mark.parametrize("ps", [1, 8, 32])
+def test_store_reports_a_batch_far_behind_the_rows(cuda, ps, new):
+    """A slice of a batch all of whose rows lie behind those of K and V: the bit,
+    and nothing written."""
+    H, D, P = 2, 64, 100
+    idx, _ = make_index([0] * len(new), new, ps, P, 1)
+    idx = idx._replace(qo_indptr=idx.qo_indptr + 5000)
+    for rows in (1, 3, 100):
+        pool = yl.quant_kv_pool(P, ps, H, D, device=cuda)
+        err = torch.zeros(1, dtype=torch.int32, device=cuda)
+        k = torch.ones(rows, H, D, dtype=torch.bfloat16, device=cuda)
+        yl.store_kv_cache_quant(k, k, pool, idx, error_word=err)
+        assert int(err.item()) == yl.DEVERR_TOKEN_COUNT
+        assert not bool(pool.k.float().any())
+
+
 @pytest.mark.parametrize("kv", ["e4m3", "16"])
 @pytest.mark.parametrize("new,have", [(10, 5), (3, 1), (90, 60), (90, 3), (90, 89)])
 @pytest.mark.parametrize("window", [0, 9])

@@ -19,8 +19,8 @@
 // plain copy; a decode step of 256 sequences, 32 layers, 22.3 us, 2.3 TB/s (two
 // rounds of eight planes a warp, and 213 instructions per 512 bytes of rows, 60 %
 // of the issue slots); pages of one token 937 us for the same prompts; 131,072
-// tokens of one layer read back in 154 us, 5.2 TB/s, where two bytes in three are writes and
-// a fill of the same memory reaches 3.9 TB/s.
+// tokens of one layer read back in 154 us, 5.2 TB/s, where two bytes in three are
+// writes and a fill of the same memory reaches 3.9 TB/s.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -48,7 +48,7 @@ struct QuantStoreParams {
   int64_t indices_cap, num_tokens;
   uint32_t *error_word;
   int32_t batch, planes;
-  uint32_t cands, chunks, runs, planes_per_run, last_row;
+  uint32_t cands, chunks, runs, planes_per_run;
 };
 
 constexpr int kStoreThreads = 128;
@@ -65,9 +65,10 @@ struct Touched {
   int count;     // new tokens of the page; 0: nothing to do
 };
 
-// By token, rows that k and v lack are nobody's number: the number of their last
-// row looks for them.  (A call of its own: the two compares inline cost a decode
-// step of 256 sequences 0.2 us, a warp beyond the units 0.3 of 22.4.)
+// Rows that k and v lack may be nobody's number: the last number, found in
+// sequence i, which ends at row q1, looks for them.  (A call of its own: the two
+// compares inline cost a decode step of 256 sequences 0.2 us, a warp beyond the
+// units 0.3 of 22.4.)
 __device__ __noinline__ void look_behind(const QuantStoreParams &p, int64_t q1, int i) {
   if (q1 > p.num_tokens || (i + 1 < p.batch && __ldg(p.qo_indptr + p.batch) > p.num_tokens))
     raise_deverr(p.error_word, YL_DEVERR_TOKEN_COUNT);
@@ -102,7 +103,7 @@ __device__ __forceinline__ Touched find_page(const QuantStoreParams &p, uint32_t
     });
     load();
   }
-  if (BY_TOKEN && cand == p.last_row) look_behind(p, q1, i);
+  if (cand + 1 == p.cands) look_behind(p, q1, i);
   const int64_t fresh = q1 - q0, pages = e1 - e0;
   if (fresh <= 0 || q0 < 0) return r;
   last = min(max(last, 0), ps);
@@ -668,7 +669,6 @@ extern "C" int yl_kv_quant_store(const yl_quant_store_args *a, cudaStream_t stre
   p.num_tokens = a->num_tokens;
   p.error_word = a->error_word;
   p.batch = a->batch_size;
-  p.last_row = static_cast<uint32_t>(a->num_tokens - 1);
   p.planes = 2 * a->pool.num_layers;
   const int64_t by_page = a->num_tokens / a->pool.page_size + 2ll * a->batch_size;
   const bool by_token = a->num_tokens <= by_page;
